@@ -14,11 +14,13 @@ LAYOUT_TILE, LAYOUT_FAST = 0, 1
 PATH_AUTO, PATH_GEMV, PATH_TCGEN05, PATH_TCGEN05_F8 = 0, 1, 2, 3
 FLAG_ACCUMULATE, FLAG_PDL, FLAG_ATOMIC = 1, 2, 4
 X_F16, X_F32, X_F32_SILU_MUL = 0, 1, 2
-STATUS_WAIT_TIMEOUT, STATUS_BAD_CODEBOOK, STATUS_BAD_SMEM = 1, 2, 4
+STATUS_WAIT_TIMEOUT, STATUS_BAD_CODEBOOK, STATUS_BAD_SMEM, STATUS_BAD_PAGE = 1, 2, 4, 8
+T_F32, T_F16, T_BF16 = 0, 1, 2
 
 EXPORTS = (
     "dmm_i8", "dmm_f16", "dmm_f16_fused", "dmm_f16_fused_tp", "dmm_f16_tp_produce", "dmm_f16_tp_consume", "dmm_tp_finalize", "dmm_xrank_barrier", "dmm_xrank_allreduce_add", "dmm_f16_chain", "dmm_f16_sequence", "dmm_f16_noalloc", "dmm_decode", "dmm_workspace_bytes", "dmm_status", "dmm_select_path",
     "dmm_hint_next_weights", "dmm_set_wait_limit_ms", "dmm_launch_count", "dmm_error_string", "dmm_version",
+    "dmm_append_kv", "dmm_paged_attention", "dmm_prompt_attention", "dmm_attention_workspace_bytes",
 )
 
 
@@ -37,6 +39,14 @@ class FusedOp(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("x_kind", ctypes.c_int), ("x_ld", ctypes.c_int64), ("x_gap", ctypes.c_int64),
                 ("codes", ctypes.c_void_p), ("cb16", ctypes.c_void_p), ("scale", ctypes.c_float), ("out", ctypes.c_void_p),
                 ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("zero_ptr", ctypes.c_void_p), ("zero_count", ctypes.c_int64)]
+
+
+class PagedCacheArg(ctypes.Structure):
+    """``dmm_paged_cache`` of include/dmm.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("table_stride", ctypes.c_int64), ("type", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("num_seqs", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
 
 
 def lib() -> ctypes.CDLL:
@@ -91,6 +101,15 @@ def lib() -> ctypes.CDLL:
     L.dmm_hint_next_weights.restype = ci
     L.dmm_set_wait_limit_ms.argtypes = [cu]
     L.dmm_set_wait_limit_ms.restype = ci
+    cf = ctypes.c_float
+    L.dmm_append_kv.argtypes = [vp, ci, i64, i64, ci, vp, ci, vp, i64, vp, vp, cu, vp]
+    L.dmm_append_kv.restype = ci
+    L.dmm_paged_attention.argtypes = [vp, i64, ci, cf, vp, i64, vp, vp, sz, cu, vp]
+    L.dmm_paged_attention.restype = ci
+    L.dmm_prompt_attention.argtypes = [vp, i64, i64, ci, cf, vp, i64, vp, vp, vp, sz, cu, vp]
+    L.dmm_prompt_attention.restype = ci
+    L.dmm_attention_workspace_bytes.argtypes = [i64, ci, ci, ci, ci]
+    L.dmm_attention_workspace_bytes.restype = sz
     L.dmm_launch_count.argtypes = []
     L.dmm_launch_count.restype = ctypes.c_uint64
     L.dmm_error_string.argtypes = [ci]

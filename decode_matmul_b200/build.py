@@ -1,11 +1,13 @@
 """Builds libdmm.so (the CUDA library behind the C ABI in include/dmm.h) with nvcc for sm_100a.
 
-The library is a single translation unit, csrc/dmm_api.cu, which includes the kernel
-headers; the result is written next to this file so that it travels with the source tree.
+The library has two translation units, csrc/dmm_api.cu (the products) and csrc/dmm_attn_api.cu (attention), which
+include the kernel headers and are compiled side by side; the result is written next to this file so that it travels
+with the source tree.  The object files stay there too, and one whose sources have not changed is taken as it is.
 """
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -13,11 +15,12 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdmm.so")
+UNITS = ("dmm_api.cu", "dmm_attn_api.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -27,6 +30,18 @@ def sources():
         out += [os.path.join(root, f) for f in files if f.endswith((".cu", ".cuh", ".h"))]
     out.append(os.path.join(HERE, "..", "include", "dmm.h"))
     return out
+
+
+def _depends(path, seen=None):
+    """A source file and everything of this library that it includes."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^#include "([^"]+)"', f.read(), re.M):
+                _depends(os.path.join(os.path.dirname(path), name), seen)
+    return seen
 
 
 def needs_build() -> bool:
@@ -52,19 +67,36 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if not force and not needs_build():
                 return LIB
             nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+            objects, running, log = [], [], ""
+            for unit in UNITS:
+                source = os.path.join(CSRC, unit)
+                obj = source[:-3] + ".o"
+                objects.append(obj)
+                if not force and os.path.exists(obj) and all(os.path.getmtime(s) <= os.path.getmtime(obj) for s in _depends(source)):
+                    continue
+                tmp = f"{obj}.{os.getpid()}.tmp"
+                cmd = [nvcc, *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-c", "-o", tmp, source]
+                running.append((obj, tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+            failed = False
+            for obj, tmp, proc in running:
+                log += proc.communicate()[0]
+                if proc.returncode == 0:
+                    os.replace(tmp, obj)
+                    continue
+                failed = True
+                if os.path.exists(tmp):
+                    os.remove(tmp)
+            if failed:
+                raise RuntimeError("nvcc failed:\n" + log)
             tmp = f"{LIB}.{os.getpid()}.tmp"
-            cmd = [nvcc, *NVCC_FLAGS, "-o", tmp, os.path.join(CSRC, "dmm_api.cu")]
-            if verbose:
-                cmd.insert(1, "-Xptxas")
-                cmd.insert(2, "-v")
-            res = subprocess.run(cmd, capture_output=True, text=True)
+            res = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", tmp, *objects], capture_output=True, text=True)
             if res.returncode != 0:
                 if os.path.exists(tmp):
                     os.remove(tmp)
                 raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
             os.replace(tmp, LIB)
             if verbose:
-                sys.stderr.write(res.stderr)
+                sys.stderr.write(log)
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
     return LIB

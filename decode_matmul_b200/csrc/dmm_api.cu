@@ -1,6 +1,6 @@
 // C ABI of libdmm (declared in include/dmm.h): argument validation, workspace and
-// per-device state, path selection, kernel launches.  The whole library is this one
-// translation unit; the kernel headers are included below.
+// per-device state, path selection, kernel launches.  The products are this translation
+// unit, with the kernel headers included below; the attention operators are dmm_attn_api.cu.
 #include <atomic>
 #include <mutex>
 
@@ -28,7 +28,7 @@ struct DeviceState {
 
 static std::mutex g_mutex;
 static DeviceState g_dev[kMaxDevices];
-static std::atomic<uint64_t> g_launches{0};
+std::atomic<uint64_t> g_launches{0};
 // dmm_hint_next_weights: what the calling host thread said its next-but-one product will stream
 struct NextHint {
     const void *codes = nullptr;
@@ -885,11 +885,10 @@ int dmm_status(unsigned *status_out) {
     cudaError_t err = cudaDeviceSynchronize();
     if (err != cudaSuccess) return err;
     unsigned v = 0;
-    err = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
-    if (err != cudaSuccess) return err;
-    const unsigned zero = 0;
-    err = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
-    if (err != cudaSuccess) return err;
+    int rc = take_status(&v);
+    if (rc) return rc;
+    rc = take_attention_status(&v);
+    if (rc) return rc;
     if (v != 0) {
         // a chain that gave up may have left its arrival counters behind
         DeviceState *d = nullptr;
@@ -965,8 +964,8 @@ const char *dmm_error_string(int code) {
     switch (code) {
         case DMM_OK: return "ok";
         case DMM_ERR_NULL: return "a required pointer is NULL";
-        case DMM_ERR_SHAPE: return "bad shape: need M >= 1, N % 16 == 0, K % 32 == 0";
-        case DMM_ERR_ALIGN: return "a pointer is not 16-byte aligned";
+        case DMM_ERR_SHAPE: return "bad shape (products need M >= 1, N % 16 == 0, K % 32 == 0)";
+        case DMM_ERR_ALIGN: return "a pointer or stride is not 16-byte aligned";
         case DMM_ERR_ARG: return "unknown enum value";
         case DMM_ERR_WORKSPACE: return "workspace too small (see dmm_workspace_bytes)";
         case DMM_ERR_UNSUPPORTED: return "shape or layout not implemented by the chosen path";

@@ -1,0 +1,95 @@
+// What the attention kernels share: 16-bit types, the view of a paged cache, and the way from a row of packed tokens to its
+// sequence and position.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dmm_common.cuh"
+
+namespace dmm {
+
+// two floats rounded to one word of two 16-bit values, a in the low half
+template <class T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <class T>
+__device__ __forceinline__ float2 unpack16(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack16<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t w) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
+}
+
+// The cache as the kernels see it (dmm_paged_cache).
+struct CacheView {
+    void *k, *v;
+    const int32_t *page_table;
+    const int32_t *seq_lens;
+    long long page_stride, head_stride, row_stride, table_stride;
+    int num_pages, kv_heads, page_shift, num_seqs, max_pages;
+};
+
+// Length of sequence b, within what its row of the page table can hold.
+__device__ __forceinline__ int cache_len(const CacheView &c, int b) {
+    const int len = c.seq_lens[b];
+    const long long most = static_cast<long long>(c.max_pages) << c.page_shift;
+    if (len >= 0 && len <= most) return len;
+    raise_status(DMM_STATUS_BAD_PAGE);
+    return len < 0 ? 0 : static_cast<int>(most);
+}
+
+// Offset (in elements) of the row of token `pos` of sequence b, head h; -1 when the table names a page that the cache does not have.
+__device__ __forceinline__ long long cache_row(const CacheView &c, int b, int pos, int h) {
+    const int page = c.page_table[b * c.table_stride + (pos >> c.page_shift)];
+    if (page < 0 || page >= c.num_pages) {
+        raise_status(DMM_STATUS_BAD_PAGE);
+        return -1;
+    }
+    return page * c.page_stride + h * c.head_stride + (pos & ((1 << c.page_shift) - 1)) * c.row_stride;
+}
+
+// The rows of sequence b among the packed tokens: [begin, begin + n).
+struct TokenSpan {
+    int begin, n;
+};
+__device__ __forceinline__ TokenSpan token_span(const int32_t *cu, int b, int tokens) {
+    if (cu == nullptr) return {b, b < tokens ? 1 : 0};
+    const int c0 = cu[b], c1 = cu[b + 1];
+    if (c0 < 0 || c1 < c0 || c1 > tokens) {
+        raise_status(DMM_STATUS_BAD_PAGE);
+        return {0, 0};
+    }
+    return {c0, c1 - c0};
+}
+
+// The sequence that row t of the packed tokens belongs to, -1 behind the last one.  Called by every thread of a block of NT
+// threads; *found is a word of shared memory.
+template <int NT>
+__device__ __forceinline__ int token_sequence(const int32_t *cu, int num_seqs, int tokens, int t, int *found) {
+    if (cu == nullptr) return t < num_seqs ? t : -1;
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    for (int b = threadIdx.x; b < num_seqs; b += NT) {
+        const TokenSpan s = token_span(cu, b, tokens);
+        if (s.begin <= t && t - s.begin < s.n) *found = b;
+    }
+    __syncthreads();
+    return *found;
+}
+
+}  // namespace dmm

@@ -11,12 +11,24 @@ namespace dmm {
 
 // ---------------------------------------------------------------------------------------
 // Device status word (one per device that loads the library).  Kernels OR bits into it;
-// dmm_status() reads and clears it.  The library is built as a single translation unit
-// (dmm_api.cu includes every kernel header), so this is the only definition.
+// dmm_status() reads and clears it.  Each translation unit of the library has a word of its own (device code is
+// not linked across them), dmm_status() takes them together.
 // ---------------------------------------------------------------------------------------
-__device__ unsigned g_status = 0;
+static __device__ unsigned g_status = 0;
 
 __device__ __forceinline__ void raise_status(unsigned bits) { atomicOr(&g_status, bits); }
+
+// Adds this translation unit's status word of the current device to *v and clears it.
+static inline int take_status(unsigned *v) {
+    unsigned mine = 0;
+    cudaError_t err = cudaMemcpyFromSymbol(&mine, g_status, sizeof(mine));
+    if (err != cudaSuccess) return err;
+    const unsigned zero = 0;
+    err = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+    if (err != cudaSuccess) return err;
+    *v |= mine;
+    return 0;
+}
 
 // ---------------------------------------------------------------------------------------
 // PTX wrappers

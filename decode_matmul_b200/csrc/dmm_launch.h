@@ -4,7 +4,15 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace dmm {
+
+// Kernels launched in this process by any entry point (dmm_launch_count).
+extern std::atomic<uint64_t> g_launches;
+
+// The status word of the attention kernels' translation unit: added to *v and cleared (take_status).
+int take_attention_status(unsigned *v);
 
 struct StreamParams {
     const void *x;          // [M, K] int8 or fp16, row-major

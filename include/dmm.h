@@ -86,6 +86,8 @@ extern "C" {
 #define DMM_STATUS_WAIT_TIMEOUT 1u /* a bounded device-side wait expired */
 #define DMM_STATUS_BAD_CODEBOOK 2u /* codebook byte not congruent to 2 mod 4, or fp16 entry not k/4 */
 #define DMM_STATUS_BAD_SMEM 4u     /* shared-memory carve-up did not fit */
+#define DMM_STATUS_BAD_PAGE 8u     /* paged cache: a page number outside the cache, a length beyond the page table, or
+                                      cu_seqlens that do not ascend within the tokens; see dmm_paged_cache */
 
 /*
  * Integer family.  out[M,N] (int32) (+)= x[M,K] (int8) . decode(codes)[N,K]^T, exact.
@@ -334,6 +336,79 @@ int dmm_hint_next_weights(const int16_t *codes, int64_t N, int64_t K);
  * multi-GPU step, which the reference does not have.
  */
 int dmm_set_wait_limit_ms(unsigned ms);
+
+/*
+ * ------------------------------------------------------------------------------------------------
+ * Attention between the products: a paged key-value cache, what appends to it and what reads it.
+ * (No counterpart in the reference, which has one product and leaves the model around it to the caller.)
+ * ------------------------------------------------------------------------------------------------
+ */
+#define DMM_T_F32 0
+#define DMM_T_F16 1
+#define DMM_T_BF16 2
+
+/*
+ * The cache of one layer and the state of the sequences in it.  Key (and value) of token `pos` of sequence b, head h:
+ *   k + page_table[b * table_stride + pos / page_size] * page_stride + h * head_stride + (pos % page_size) * row_stride
+ * head_dim contiguous values of `type`; the strides are in elements, the same for k and v, multiples of 8, in any order of
+ * the three dimensions that lets no two rows overlap.  page_size is a power of two, 16 or more; head_dim is 64 or 128;
+ * k and v are 16-byte aligned.
+ * seq_lens[b] is the length of sequence b in tokens, those of the present call included; table entries behind a
+ * sequence's last page are not read.
+ * page_table, seq_lens and cu_seqlens are device memory, so a captured graph serves sequences as they grow.  No kernel
+ * follows what they say beyond the cache: a page number outside [0, num_pages) is not written to and reads as zeros, a
+ * length outside [0, max_pages * page_size] counts as the nearer end, sequences whose cu_seqlens descend or leave
+ * [0, tokens] as without new tokens, and DMM_STATUS_BAD_PAGE is raised.
+ */
+typedef struct dmm_paged_cache {
+    void *k, *v;
+    const int32_t *page_table; /* [num_seqs, max_pages], rows table_stride entries apart */
+    const int32_t *seq_lens;   /* [num_seqs] */
+    int64_t num_pages, page_stride, head_stride, row_stride, table_stride;
+    int32_t type;              /* DMM_T_F16 or DMM_T_BF16 */
+    int32_t kv_heads, head_dim, page_size, num_seqs, max_pages;
+} dmm_paged_cache;
+
+/*
+ * The result of a qkv product becomes queries, and new rows of the cache.  qkv: [tokens, qkv_ld] of qkv_type (fp32, fp16 or
+ * bf16), a row = `heads` query heads, then kv_heads key heads, then kv_heads value heads of head_dim values.  The tokens of
+ * sequence b are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 and its last ones: token i of n has position
+ * seq_lens[b] - n + i.  cu_seqlens (int32 [num_seqs + 1]) may be NULL: one token per sequence, row b.
+ * Queries and keys are rotated by their position: freqs[i] (double, head_dim / 2 of them, device memory) is the angle
+ * in radians per position of pair i, (a, b) -> (a cos - b sin, a sin + b cos); a pair is (i, i + head_dim / 2), or
+ * (2 i, 2 i + 1) with `interleaved`.  freqs NULL: no rotation.  The angle is reduced in 64 bits, the rotation is done in 32
+ * and rounded once to the cache's type.  q_out: [tokens, heads * head_dim] of the cache's type, rows q_ld apart.
+ * Rows of qkv behind the last sequence and tokens at negative positions (more new tokens than the length says, which
+ * raises DMM_STATUS_BAD_PAGE) are skipped: neither q_out nor the cache is written for them.  flags: DMM_FLAG_PDL only.
+ */
+int dmm_append_kv(const void *qkv, int qkv_type, int64_t qkv_ld, int64_t tokens, int heads, const double *freqs,
+                  int interleaved, void *q_out, int64_t q_ld, const dmm_paged_cache *cache, const int32_t *cu_seqlens,
+                  unsigned flags, void *stream);
+
+/*
+ * Attention of one new token per sequence: out[b, h] = sum_j softmax_j(scale * q[b, h] . k[j, h / group]) v[j, h / group]
+ * over the keys j < seq_lens[b], group = heads / kv_heads (at most 128).  q and out: [num_seqs, heads, head_dim] of
+ * the cache's type, q_ld / out_ld elements from one sequence to the next (multiples of 8), 16-byte aligned.  A sequence
+ * of length 0 gets zeros.  The keys of all sequences are cut into equal shares, one per CTA; what shares of one sequence
+ * have in common is joined in a fixed order, so equal inputs give equal bits.  workspace: scratch of
+ * dmm_attention_workspace_bytes, 256-byte aligned, of any content; calls that can overlap on the GPU need distinct ones.
+ * flags: DMM_FLAG_PDL only.
+ */
+int dmm_paged_attention(const void *q, int64_t q_ld, int heads, float scale, void *out, int64_t out_ld,
+                        const dmm_paged_cache *cache, void *workspace, size_t workspace_bytes, unsigned flags, void *stream);
+
+/*
+ * Causal attention of packed prompts, or of the next chunk of each: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q
+ * are the last tokens of sequence b, and row i of n sees the keys j <= seq_lens[b] - n + i, all of which are in the cache
+ * (dmm_append_kv has put the new ones there).  A row that sees no key gets zeros; rows behind the last sequence are left
+ * as they are.  Everything else as in dmm_paged_attention.
+ */
+int dmm_prompt_attention(const void *q, int64_t q_ld, int64_t tokens, int heads, float scale, void *out, int64_t out_ld,
+                         const dmm_paged_cache *cache, const int32_t *cu_seqlens, void *workspace,
+                         size_t workspace_bytes, unsigned flags, void *stream);
+
+/* Bytes of workspace that dmm_paged_attention (tokens = num_seqs) and dmm_prompt_attention need, for any lengths. */
+size_t dmm_attention_workspace_bytes(int64_t tokens, int num_seqs, int heads, int kv_heads, int head_dim);
 
 /* Bytes of workspace a call of dmm_i8 / dmm_f16 with these sizes needs (0 if none). */
 size_t dmm_workspace_bytes(int64_t M, int64_t N, int64_t K);
