@@ -3,6 +3,7 @@
 
 #include "dmm_attn_append.cuh"
 #include "dmm_attn_common.cuh"
+#include "dmm_attn_prompt.cuh"
 #include "dmm_attn_simple.cuh"
 #include "dmm_launch.h"
 
@@ -114,6 +115,20 @@ static int attention(const void *q, int64_t q_ld, int64_t tokens, int heads, flo
     p.scale = scale;
     const bool pdl = (flags & DMM_FLAG_PDL) != 0;
     g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (cu != nullptr) {
+        PromptParams pp = {};
+        pp.q = q;
+        pp.out = out;
+        pp.cu = cu;
+        pp.q_ld = q_ld;
+        pp.out_ld = out_ld;
+        pp.cache = p.cache;
+        pp.tokens = p.tokens;
+        pp.heads = heads;
+        pp.group = p.group;
+        pp.scale = scale;
+        return launch_prompt(pp, cache->type, cache->head_dim, pdl, stream);
+    }
     if (cache->type == DMM_T_F16)
         return cache->head_dim == 64 ? launch_attention<__half, 64>(p, pdl, stream) : launch_attention<__half, 128>(p, pdl, stream);
     return cache->head_dim == 64 ? launch_attention<__nv_bfloat16, 64>(p, pdl, stream) : launch_attention<__nv_bfloat16, 128>(p, pdl, stream);

@@ -1,0 +1,550 @@
+// Causal attention of packed prompts over a paged cache, on the 5th-generation tensor cores.
+//
+// One pass over the keys with the softmax's running maximum m and sum l: for key tiles j of 128 keys,
+//   S = Q K_j^T,  P = exp2(c S - c m),  O += P V_j,  l += rowsum(P),   result O / l,   c = scale log2(e).
+//
+// A CTA has two tiles of 128 query rows of one key head and one sequence, so that the tensor cores work for one tile while
+// the softmax of the other runs.  The rows of a tile are (token, query head of the group): all the heads that share a
+// key head read its tile once, and a tile spans few tokens, so little of the causal triangle's edge is computed in vain.
+// Tensor memory holds S of both tiles (2 x 128 columns; P, in 16 bits, takes the place of the first half of its S) and O of both.
+//   warps 0..3, 4..7   softmax of tile 0, 1: a thread has a row
+//   warp 8             MMA issue (one elected lane)
+//   warp 9             TMA loads: Q, then K_0, V_0, K_1, ...; a tile of keys is one box per page
+//   warps 10, 11       guard: rows of V behind the sequence's end become zeros in shared memory (0 * garbage could be NaN), and
+//                      values that are not finite too where a row of the tile must not see them; the epilogue then adds
+//                      them to the rows that do see them.  Only tiles in which a row ends are looked at.
+// O is only brought to a new maximum when that has risen by more than 2^8 (c (max - m) > 8): the weights stay below
+// 2^8, far from overflow, and the quotient O / l is the same.
+#pragma once
+
+#include "dmm_attn_common.cuh"
+#include "dmm_tmem.cuh"
+
+namespace dmm {
+
+struct PromptParams {
+    const void *q;
+    void *out;
+    const int32_t *cu;
+    long long q_ld, out_ld;
+    CacheView cache;
+    int tokens, heads, group, tile_tokens;  // tile_tokens = 128 / group: tokens of a tile
+    float scale;
+};
+
+constexpr int kPromptThreads = 384;
+constexpr int kPromptKeys = 128;  // keys of a tile
+
+// Key tiles in which rows of a pair of tiles end: they are 256 tokens at most.
+constexpr int kMostGuarded = 3;
+
+template <int D>
+struct PromptPlan {
+    static constexpr int kHalves = D / 64;            // columns of 128 bytes that a tile consists of
+    static constexpr uint32_t kHalfBytes = 128 * 128; // 128 rows of 128 bytes
+    static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
+    static constexpr int kStages = D == 128 ? 5 : 8;
+    static constexpr uint32_t kQ = 0;
+    static constexpr uint32_t kRing = 2 * kTileBytes;
+    static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
+    static constexpr int kBarQ = 0, kBarFull = 2, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarP = kBarS + 2,
+                         kBarO = kBarP + 2, kBarGuard = kBarO + 2, kBarLook = kBarGuard + 1, kNumBars = kBarLook + kMostGuarded;
+    static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 64 + 1024;  // (the last: alignment)
+    static constexpr uint32_t kS = 0, kO = 256;       // tensor memory columns: S of tile i at 128 i, O at 256 + D i
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *tmap, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem], descriptors as low and high words
+__device__ __forceinline__ void mma_ss_f16(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %6, 0;\nmov.b64 ad, {%1, %2};\nmov.b64 bd, {%3, %4};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %5, p;\n}\n" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts_f16_words(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 bd;\nsetp.ne.b32 p, %5, 0;\nmov.b64 bd, {%2, %3};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
+    uint32_t u[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+          "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+          "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// What a CTA works on.
+struct PromptItem {
+    int seq, head, begin, n, len, token0;  // token0: first token of tile 0 within the sequence's new tokens
+};
+
+// Item `index` in the order: sequences as they come, tile pairs from the last (which has the most keys) to the first,
+// key heads innermost.  By the lanes of one warp; seq = -1 when there is no such item.
+__device__ __forceinline__ PromptItem prompt_item(const PromptParams &p, int index) {
+    const int lane = threadIdx.x & 31, span_tokens = 2 * p.tile_tokens;
+    PromptItem it = {-1, index % p.cache.kv_heads, 0, 0, 0, 0};
+    int rest = index / p.cache.kv_heads;
+    for (int b0 = 0; b0 < p.cache.num_seqs; b0 += 32) {
+        const int b = b0 + lane;
+        TokenSpan s = {0, 0};
+        if (b < p.cache.num_seqs) s = token_span(p.cu, b, p.tokens);
+        const int pairs = (s.n + span_tokens - 1) / span_tokens;
+        int upto = pairs;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned after = __ballot_sync(0xffffffffu, upto > rest);
+        if (after != 0) {
+            const int who = __ffs(after) - 1;
+            it.seq = b0 + who;
+            it.begin = __shfl_sync(0xffffffffu, s.begin, who);
+            it.n = __shfl_sync(0xffffffffu, s.n, who);
+            const int at = rest - __shfl_sync(0xffffffffu, upto - pairs, who);
+            it.token0 = (__shfl_sync(0xffffffffu, pairs, who) - 1 - at) * span_tokens;
+            it.len = cache_len(p.cache, it.seq);
+            return it;
+        }
+        rest -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return it;
+}
+
+template <class T>
+struct F16Kind;  // operand type bits of the instruction descriptor; a word whose 16-bit halves are all exponent
+template <>
+struct F16Kind<__half> {
+    static constexpr uint32_t kType = 0, kExponent = 0x7C00u;
+};
+template <>
+struct F16Kind<__nv_bfloat16> {
+    static constexpr uint32_t kType = (1u << 7) | (1u << 10), kExponent = 0x7F80u;
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                            const __grid_constant__ CUtensorMap vmap, const PromptParams p) {
+    using Plan = PromptPlan<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PromptItem s_item;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_failed, s_poison;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const auto bar = [&](int i) { return smem + Plan::kBars + 8u * static_cast<uint32_t>(i); };
+    grid_dep_wait();
+    if (warp == 0) {
+        const PromptItem it = prompt_item(p, static_cast<int>(blockIdx.x));
+        if (lane == 0) s_item = it;
+    } else if (warp == 8) {
+        if (lane == 0) {
+            s_failed = 0;
+            s_poison = 0;
+            for (int i = 0; i < Plan::kNumBars; ++i)
+                mbar_init(bar(i), i >= Plan::kBarP && i < Plan::kBarP + 2 ? 4 : i == Plan::kBarGuard ? 2 : 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    const PromptItem it = s_item;
+    if (it.seq < 0) return;
+    if (warp == 8) tmem_alloc(smem_u32(&s_tmem), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    // Row i of the new tokens sees keys below len - n + i + 1.  first, last: of the tokens of a tile that exist.
+    const int shift = it.len - it.n + 1, tt = p.tile_tokens;
+    const auto limit = [&](int token) { return shift + token; };
+    int tiles[2], most[2];  // key tiles, and keys that the last row sees
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t0 = it.token0 + i * tt, t1 = min(t0 + tt, it.n);
+        most[i] = t1 > t0 ? max(0, limit(t1 - 1)) : 0;
+        tiles[i] = (most[i] + kPromptKeys - 1) / kPromptKeys;
+    }
+    const int all = max(tiles[0], tiles[1]);
+    // the first key tile in which a row ends, or the sequence; the values of these tiles arrive at barriers of their own, for the guard
+    const int guarded = max(0, limit(it.token0)) / kPromptKeys;
+
+    if (warp == 9) {
+        // =============================== loads ===============================
+        if (all > 0) {
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (tiles[i] > 0) {
+                        mbar_arrive_expect_tx(bar(Plan::kBarQ + i), static_cast<uint32_t>(Plan::kHalves * p.group * tt) * 128u);
+#pragma unroll
+                        for (int hh = 0; hh < Plan::kHalves; ++hh)
+                            tma_load_3d(smem + Plan::kQ + i * Plan::kTileBytes + hh * Plan::kHalfBytes, &qmap, 64 * hh, it.head * p.group,
+                                        it.begin + it.token0 + i * tt, bar(Plan::kBarQ + i));
+                    }
+            }
+            const int shift_pg = p.cache.page_shift, page = 1 << shift_pg, box = min(page, kPromptKeys);
+            const int32_t *table = p.cache.page_table + it.seq * p.cache.table_stride;
+            int stage = 0;
+            uint32_t parity = 1;
+            for (int j = 0; j < all; ++j) {
+                const int pos = j * kPromptKeys + lane * box;
+                const bool mine = lane * box < kPromptKeys && pos < it.len;
+                int pg = 0;
+                if (mine) {
+                    pg = table[pos >> shift_pg];
+                    if (pg < 0 || pg >= p.cache.num_pages) {
+                        raise_status(DMM_STATUS_BAD_PAGE);
+                        pg = -1;  // outside the tensor map: reads as zeros
+                    }
+                }
+                const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine)) * box) * 128u * Plan::kHalves;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    mbar_wait(bar(Plan::kBarEmpty + stage), parity, &s_failed);
+                    const uint32_t full = bar(kv == 1 && j >= guarded ? Plan::kBarLook + j - guarded : Plan::kBarFull + stage);
+                    if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+                    __syncwarp();
+                    if (mine) {
+                        const uint32_t dst = smem + Plan::kRing + stage * Plan::kTileBytes + static_cast<uint32_t>(lane * box) * 128u;
+#pragma unroll
+                        for (int hh = 0; hh < Plan::kHalves; ++hh)
+                            tma_load_4d(dst + hh * Plan::kHalfBytes, kv == 0 ? &kmap : &vmap, 64 * hh, pos & (page - 1), it.head, pg, full);
+                    }
+                    if (++stage == Plan::kStages) {
+                        stage = 0;
+                        parity ^= 1u;
+                    }
+                }
+            }
+            if (s_failed) {  // a wait gave up: let the copies in flight land before the CTA goes
+                for (int j = all; j-- > 0 && j >= all - Plan::kStages;) {
+                    mbar_wait_limit(bar(Plan::kBarFull + 2 * j % Plan::kStages), static_cast<uint32_t>(2 * j / Plan::kStages) & 1u, kWaitLimitCycles);
+                    if (j >= guarded) mbar_wait_limit(bar(Plan::kBarLook + j - guarded), 0, kWaitLimitCycles);
+                    else mbar_wait_limit(bar(Plan::kBarFull + (2 * j + 1) % Plan::kStages), static_cast<uint32_t>((2 * j + 1) / Plan::kStages) & 1u, kWaitLimitCycles);
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // =============================== MMA ===============================
+        const bool leader = elect_one();
+        // D fp32 (1 at bit 4), the operands' type, N >> 3 at bit 17, M >> 4 at bit 24; V is the operand whose rows run along N (bit 16)
+        constexpr uint32_t kIdS = (1u << 4) | F16Kind<T>::kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kIdO = (1u << 4) | F16Kind<T>::kType | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
+        // 128-byte swizzle (2 at bit 61), 8-row groups 1024 bytes apart, version 1 at bit 46; the low word has the address and, for
+        // V, the distance from one 64 columns to the next
+        constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+        const auto lo = [&](uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); };
+        const auto ring = [&](int n) { return smem + Plan::kRing + static_cast<uint32_t>(n % Plan::kStages) * Plan::kTileBytes; };
+        const auto phase = [&](int n) { return static_cast<uint32_t>(n / Plan::kStages) & 1u; };
+        const auto scores = [&](int i, int j) {
+            const uint32_t a = lo(smem + Plan::kQ + i * Plan::kTileBytes, 16), b = lo(ring(2 * j), 16);
+            if (leader) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k / 4) * (Plan::kHalfBytes >> 4) + (k % 4) * 2;
+                    mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, kIdS, k > 0);
+                }
+                tc_commit(bar(Plan::kBarS + i));
+            }
+        };
+        if (all > 0) {
+            mbar_wait(bar(Plan::kBarFull), 0, &s_failed);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (tiles[i] > 0) {
+                    mbar_wait(bar(Plan::kBarQ + i), 0, &s_failed);
+                    tc_fence_after();
+                    scores(i, 0);
+                }
+            if (leader) tc_commit(bar(Plan::kBarEmpty));
+            for (int j = 0; j < all; ++j) {
+                if (j < guarded)
+                    mbar_wait(bar(Plan::kBarFull + (2 * j + 1) % Plan::kStages), phase(2 * j + 1), &s_failed);
+                else
+                    mbar_wait(bar(Plan::kBarGuard), static_cast<uint32_t>(j - guarded) & 1u, &s_failed);
+                const uint32_t v = lo(ring(2 * j + 1), Plan::kHalfBytes);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (j < tiles[i]) {
+                        mbar_wait(bar(Plan::kBarP + i), static_cast<uint32_t>(j) & 1u, &s_failed);
+                        tc_fence_after();
+                        if (leader) {
+                            // (the last tile: only the 16 keys at a time that some row sees)
+                            const int steps = min(8, (most[i] - j * kPromptKeys + 15) / 16);
+                            for (int k = 0; k < steps; ++k)
+                                mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * k, v + k * (2048u >> 4), kHi, kIdO, j > 0 || k > 0);
+                            if (j + 1 == tiles[i]) tc_commit(bar(Plan::kBarO + i));
+                        }
+                        __syncwarp();
+                    }
+                    if (j + 1 < tiles[i]) {
+                        mbar_wait(bar(Plan::kBarFull + (2 * j + 2) % Plan::kStages), phase(2 * j + 2), &s_failed);
+                        tc_fence_after();
+                        scores(i, j + 1);
+                    }
+                }
+                if (leader) {
+                    tc_commit(bar(Plan::kBarEmpty + (2 * j + 1) % Plan::kStages));
+                    if (j + 1 < all) tc_commit(bar(Plan::kBarEmpty + (2 * j + 2) % Plan::kStages));
+                }
+            }
+        }
+    } else if (warp >= 10) {
+        // =============================== guard ===============================
+        const int t = threadIdx.x - 320;
+        constexpr uint32_t kMask = F16Kind<T>::kExponent * 0x10001u;
+        for (int j = guarded; j < all; ++j) {
+            const int n = 2 * j + 1, rows = min(kPromptKeys, it.len - j * kPromptKeys);
+            mbar_wait(bar(Plan::kBarLook + j - guarded), 0, &s_failed);
+            const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>(n % Plan::kStages) * Plan::kTileBytes;
+            const auto where = [&](int c) { return base + (c / 1024) * Plan::kHalfBytes + (c % 1024) * 16u; };  // piece c: row (c % 1024) / 8
+            const auto bad = [](uint32_t w) { return (w & 0xFFFFu & kMask) == (kMask & 0xFFFFu) || (w & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u); };
+            bool any = false;
+            for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
+                const int row = (c % 1024) / 8;
+                if (row < rows) {
+                    const uint4 w = lds128(where(c));
+                    any |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+                } else if (row < ((rows + 15) & ~15)) {
+                    sts128(where(c), make_uint4(0, 0, 0, 0));
+                }
+            }
+            if (any) {
+                s_poison = 1;
+                for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
+                    if ((c % 1024) / 8 >= rows) continue;
+                    const uint4 w = lds128(where(c));
+                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if ((x[i] & 0xFFFFu & kMask) == (kMask & 0xFFFFu)) x[i] &= 0xFFFF0000u;
+                        if ((x[i] & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u)) x[i] &= 0xFFFFu;
+                    }
+                    sts128(where(c), make_uint4(x[0], x[1], x[2], x[3]));
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Plan::kBarGuard));
+        }
+    } else {
+        // =============================== softmax ===============================
+        const int i = warp / 4, r = threadIdx.x % 128, tok = r / p.group;
+        const int token = it.token0 + i * tt + tok;
+        const bool mine = tok < tt && token < it.n;
+        const int sees = mine ? max(0, limit(token)) : 0;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
+        const uint32_t s_at = lanes + Plan::kS + 128 * i, o_at = lanes + Plan::kO + D * i;
+        // c S <= 0 for c <= 0: such scales turn the sign of S, or make it 0
+        const float turn = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
+        const float c = turn == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
+        const int free = max(0, limit(it.token0 + i * tt)) / kPromptKeys;  // key tiles that every row of this tile sees whole
+        float m = -INFINITY, l = 0.0f;
+        for (int j = 0; j < tiles[i]; ++j) {
+            mbar_wait(bar(Plan::kBarS + i), static_cast<uint32_t>(j) & 1u, &s_failed);
+            tc_fence_after();
+            const int rel = sees - j * kPromptKeys;
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float s[32];
+                tmem_ld32(s_at + 32 * q, s);
+                if (turn != 1.0f)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) s[x] *= turn;
+                if (j >= free)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) s[x] = 32 * q + x < rel ? s[x] : -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 32; ++x) top = fmaxf(top, s[x]);
+            }
+            const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
+            if (__any_sync(0xffffffffu, rise)) {
+                const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_approx((m - to) * c);
+                m = to;
+                l *= f;
+                if (j > 0) {
+#pragma unroll
+                    for (int q = 0; q < D / 16; ++q) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + 16 * q, o);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tmem_st16(o_at + 16 * q, o);
+                    }
+                }
+            }
+            const float mc = m == -INFINITY ? 0.0f : m * c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float s[32];
+                tmem_ld32(s_at + 32 * q, s);
+                if (turn != 1.0f)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) s[x] *= turn;
+                if (j >= free)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) s[x] = 32 * q + x < rel ? s[x] : -INFINITY;
+                uint32_t w[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float a = exp2_approx(fmaf(s[2 * x], c, -mc)), b = exp2_approx(fmaf(s[2 * x + 1], c, -mc));
+                    l += a + b;
+                    w[x] = pack16<T>(a, b);
+                }
+                tmem_st16(s_at + 16 * q, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Plan::kBarP + i));
+        }
+        if (tiles[i] > 0) {
+            mbar_wait(bar(Plan::kBarO + i), 0, &s_failed);
+            tc_fence_after();
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + r % p.group) * D;
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+            float o[32];
+            if (tiles[i] > 0) {
+                tmem_ld32(o_at + 32 * q, o);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = 0.0f;
+            }
+            if (s_poison && mine) {
+                for (int pos = guarded * kPromptKeys; pos < sees; ++pos) {
+                    const long long row = cache_row(p.cache, it.seq, pos, it.head);
+                    if (row < 0) continue;
+                    const T *v = static_cast<const T *>(p.cache.v) + row + 32 * q;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) {
+                        const float f = static_cast<float>(v[x]);
+                        if (!isfinite(f)) o[x] += f;
+                    }
+                }
+            }
+            if (mine) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) y[z] = o[x + z] * inv;
+                    *reinterpret_cast<uint4 *>(out + 32 * q + x) =
+                        make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Tensor maps of the queries (rows of heads) and of keys or values (pages), 128-byte swizzle, boxes 64 values wide.
+inline int make_attn_map(CUtensorMap *map, int type, const void *base, int rank, const cuuint64_t *dim, const cuuint64_t *stride, const cuuint32_t *box) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, type == DMM_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+                          const_cast<void *>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : cudaErrorInvalidValue;
+}
+
+template <class T, int D>
+inline int launch_prompt_typed(PromptParams &p, int type, bool pdl, cudaStream_t stream) {
+    using Plan = PromptPlan<D>;
+    p.tile_tokens = 128 / p.group;
+    CUtensorMap maps[3];
+    {
+        const cuuint64_t dim[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.tokens)};
+        const cuuint64_t stride[2] = {2ull * D, 2ull * static_cast<cuuint64_t>(p.q_ld)};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.tile_tokens)};
+        const int rc = make_attn_map(&maps[0], type, p.q, 3, dim, stride, box);
+        if (rc) return rc;
+    }
+    const int page = 1 << p.cache.page_shift;
+    for (int kv = 0; kv < 2; ++kv) {
+        const cuuint64_t dim[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(p.cache.kv_heads),
+                                   static_cast<cuuint64_t>(p.cache.num_pages)};
+        // (the stride of a dimension of size 1 says nothing)
+        const auto bytes = [](long long s, long long n) { return 2ull * static_cast<cuuint64_t>(n > 1 ? s : D); };
+        const cuuint64_t stride[3] = {bytes(p.cache.row_stride, page), bytes(p.cache.head_stride, p.cache.kv_heads),
+                                      bytes(p.cache.page_stride, p.cache.num_pages)};
+        const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < kPromptKeys ? page : kPromptKeys), 1, 1};
+        const int rc = make_attn_map(&maps[1 + kv], type, kv ? p.cache.v : p.cache.k, 4, dim, stride, box);
+        if (rc) return rc;
+    }
+    // every sequence adds at most one pair of tiles that is not full
+    const long long items = (p.tokens / (2 * p.tile_tokens) + static_cast<long long>(p.cache.num_seqs < p.tokens ? p.cache.num_seqs : p.tokens)) * p.cache.kv_heads;
+    if (items > 0x7fffffff) return DMM_ERR_SHAPE;
+    const auto kernel = prompt_attention_kernel<T, D>;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (!ready[dev]) {
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Plan::kBytes));
+        if (err != cudaSuccess) return err;
+        ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items));
+    cfg.blockDim = dim3(kPromptThreads);
+    cfg.dynamicSmemBytes = Plan::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
+}
+
+inline int launch_prompt(PromptParams &p, int type, int head_dim, bool pdl, cudaStream_t stream) {
+    if (type == DMM_T_F16) return head_dim == 64 ? launch_prompt_typed<__half, 64>(p, type, pdl, stream) : launch_prompt_typed<__half, 128>(p, type, pdl, stream);
+    return head_dim == 64 ? launch_prompt_typed<__nv_bfloat16, 64>(p, type, pdl, stream) : launch_prompt_typed<__nv_bfloat16, 128>(p, type, pdl, stream);
+}
+
+}  // namespace dmm
