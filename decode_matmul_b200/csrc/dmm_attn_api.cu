@@ -3,8 +3,8 @@
 
 #include "dmm_attn_append.cuh"
 #include "dmm_attn_common.cuh"
+#include "dmm_attn_decode.cuh"
 #include "dmm_attn_prompt.cuh"
-#include "dmm_attn_simple.cuh"
 #include "dmm_launch.h"
 
 namespace dmm {
@@ -87,11 +87,10 @@ static int check_rows(const void *p, long long ld, long long width) {
     return ld % 8 != 0 ? DMM_ERR_ALIGN : 0;
 }
 
-static int attention(const void *q, int64_t q_ld, int64_t tokens, int heads, float scale, void *out, int64_t out_ld,
-                     const dmm_paged_cache *cache, const int32_t *cu, void *workspace, size_t workspace_bytes, unsigned flags,
-                     cudaStream_t stream) {
-    AttnParams p = {};
-    int rc = cache_view(cache, &p.cache);
+// What both attention entries check.
+static int check_attention(const void *q, int64_t q_ld, int64_t tokens, int heads, const void *out, int64_t out_ld,
+                           const dmm_paged_cache *cache, CacheView *view, const void *workspace, size_t workspace_bytes, unsigned flags) {
+    int rc = cache_view(cache, view);
     if (rc) return rc;
     if (heads < 1 || heads % cache->kv_heads != 0 || heads / cache->kv_heads > 128) return DMM_ERR_SHAPE;
     if (tokens < 1 || tokens > 0x7fffffff || heads > 65535) return DMM_ERR_SHAPE;
@@ -102,36 +101,8 @@ static int attention(const void *q, int64_t q_ld, int64_t tokens, int heads, flo
     if (rc) return rc;
     if (flags & ~DMM_FLAG_PDL) return DMM_ERR_ARG;
     const size_t need = dmm_attention_workspace_bytes(tokens, cache->num_seqs, heads, cache->kv_heads, cache->head_dim);
-    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return DMM_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return DMM_ERR_ALIGN;
-    p.q = q;
-    p.out = out;
-    p.cu = cu;
-    p.q_ld = q_ld;
-    p.out_ld = out_ld;
-    p.tokens = static_cast<int>(tokens);
-    p.heads = heads;
-    p.group = heads / cache->kv_heads;
-    p.scale = scale;
-    const bool pdl = (flags & DMM_FLAG_PDL) != 0;
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    if (cu != nullptr) {
-        PromptParams pp = {};
-        pp.q = q;
-        pp.out = out;
-        pp.cu = cu;
-        pp.q_ld = q_ld;
-        pp.out_ld = out_ld;
-        pp.cache = p.cache;
-        pp.tokens = p.tokens;
-        pp.heads = heads;
-        pp.group = p.group;
-        pp.scale = scale;
-        return launch_prompt(pp, cache->type, cache->head_dim, pdl, stream);
-    }
-    if (cache->type == DMM_T_F16)
-        return cache->head_dim == 64 ? launch_attention<__half, 64>(p, pdl, stream) : launch_attention<__half, 128>(p, pdl, stream);
-    return cache->head_dim == 64 ? launch_attention<__nv_bfloat16, 64>(p, pdl, stream) : launch_attention<__nv_bfloat16, 128>(p, pdl, stream);
+    if (workspace == nullptr || workspace_bytes < need) return DMM_ERR_WORKSPACE;
+    return reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ? DMM_ERR_ALIGN : 0;
 }
 
 }  // namespace dmm
@@ -176,23 +147,55 @@ int dmm_append_kv(const void *qkv, int qkv_type, int64_t qkv_ld, int64_t tokens,
 }
 
 size_t dmm_attention_workspace_bytes(int64_t tokens, int num_seqs, int heads, int kv_heads, int head_dim) {
-    (void)tokens, (void)num_seqs, (void)heads, (void)kv_heads, (void)head_dim;
-    return 0;
+    (void)tokens, (void)num_seqs, (void)heads, (void)kv_heads;
+    int sms = 0;
+    if (device_sms(&sms) != 0 || sms < 1) sms = 256;
+    return decode_workspace(head_dim, sms);
 }
 
 int dmm_paged_attention(const void *q, int64_t q_ld, int heads, float scale, void *out, int64_t out_ld,
                         const dmm_paged_cache *cache, void *workspace, size_t workspace_bytes, unsigned flags, void *stream) {
     if (!cache) return DMM_ERR_NULL;
-    return attention(q, q_ld, cache->num_seqs, heads, scale, out, out_ld, cache, nullptr, workspace, workspace_bytes, flags,
-                     static_cast<cudaStream_t>(stream));
+    DecodeParams p = {};
+    int rc = check_attention(q, q_ld, cache->num_seqs, heads, out, out_ld, cache, &p.cache, workspace, workspace_bytes, flags);
+    if (rc) return rc;
+    int sms = 0;
+    rc = device_sms(&sms);
+    if (rc) return rc;
+    p.q = q;
+    p.out = out;
+    p.partial = static_cast<float *>(workspace);
+    p.q_ld = q_ld;
+    p.out_ld = out_ld;
+    p.group = heads / cache->kv_heads;
+    p.q_tiles = (p.group + 15) / 16;
+    p.scale = scale;
+    const bool pdl = (flags & DMM_FLAG_PDL) != 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    g_launches.fetch_add(2, std::memory_order_relaxed);
+    if (cache->type == DMM_T_F16)
+        return cache->head_dim == 64 ? launch_decode<__half, 64>(p, sms, pdl, st) : launch_decode<__half, 128>(p, sms, pdl, st);
+    return cache->head_dim == 64 ? launch_decode<__nv_bfloat16, 64>(p, sms, pdl, st) : launch_decode<__nv_bfloat16, 128>(p, sms, pdl, st);
 }
 
 int dmm_prompt_attention(const void *q, int64_t q_ld, int64_t tokens, int heads, float scale, void *out, int64_t out_ld,
                          const dmm_paged_cache *cache, const int32_t *cu_seqlens, void *workspace,
                          size_t workspace_bytes, unsigned flags, void *stream) {
     if (!cu_seqlens) return DMM_ERR_NULL;
-    return attention(q, q_ld, tokens, heads, scale, out, out_ld, cache, cu_seqlens, workspace, workspace_bytes, flags,
-                     static_cast<cudaStream_t>(stream));
+    PromptParams p = {};
+    const int rc = check_attention(q, q_ld, tokens, heads, out, out_ld, cache, &p.cache, workspace, workspace_bytes, flags);
+    if (rc) return rc;
+    p.q = q;
+    p.out = out;
+    p.cu = cu_seqlens;
+    p.q_ld = q_ld;
+    p.out_ld = out_ld;
+    p.tokens = static_cast<int>(tokens);
+    p.heads = heads;
+    p.group = heads / cache->kv_heads;
+    p.scale = scale;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return launch_prompt(p, cache->type, cache->head_dim, (flags & DMM_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

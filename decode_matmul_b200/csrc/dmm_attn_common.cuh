@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "dmm_common.cuh"
 
 namespace dmm {
@@ -34,6 +36,28 @@ template <>
 __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t w) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
 }
+
+// 2^x, off by 2^-22 at most
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Lets a kernel have more than 48 KB of dynamic shared memory, once per device.
+struct SmemAllowance {
+    std::atomic<bool> given[64];
+    int get(const void *kernel, unsigned bytes) {
+        int dev = 0;
+        cudaError_t err = cudaGetDevice(&dev);
+        if (err != cudaSuccess) return err;
+        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+        if (given[dev].load(std::memory_order_relaxed)) return 0;
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+        if (err == cudaSuccess) given[dev].store(true, std::memory_order_relaxed);
+        return err;
+    }
+};
 
 // The cache as the kernels see it (dmm_paged_cache).
 struct CacheView {

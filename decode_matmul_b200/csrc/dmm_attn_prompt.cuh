@@ -98,12 +98,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
     for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // What a CTA works on.
 struct PromptItem {
     int seq, head, begin, n, len, token0;  // token0: first token of tile 0 within the sequence's new tokens
@@ -394,7 +388,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
             if (__any_sync(0xffffffffu, rise)) {
-                const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_approx((m - to) * c);
+                const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
                 m = to;
                 l *= f;
                 if (j > 0) {
@@ -423,7 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 uint32_t w[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float a = exp2_approx(fmaf(s[2 * x], c, -mc)), b = exp2_approx(fmaf(s[2 * x + 1], c, -mc));
+                    const float a = exp2_fast(fmaf(s[2 * x], c, -mc)), b = exp2_fast(fmaf(s[2 * x + 1], c, -mc));
                     l += a + b;
                     w[x] = pack16<T>(a, b);
                 }
@@ -520,15 +514,9 @@ inline int launch_prompt_typed(PromptParams &p, int type, bool pdl, cudaStream_t
     const long long items = (p.tokens / (2 * p.tile_tokens) + static_cast<long long>(p.cache.num_seqs < p.tokens ? p.cache.num_seqs : p.tokens)) * p.cache.kv_heads;
     if (items > 0x7fffffff) return DMM_ERR_SHAPE;
     const auto kernel = prompt_attention_kernel<T, D>;
-    static bool ready[64] = {};
-    int dev = 0;
-    cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess) return err;
-    if (!ready[dev]) {
-        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Plan::kBytes));
-        if (err != cudaSuccess) return err;
-        ready[dev] = true;
-    }
+    static SmemAllowance allowance;
+    const int rc = allowance.get(reinterpret_cast<const void *>(kernel), Plan::kBytes);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items));
     cfg.blockDim = dim3(kPromptThreads);
