@@ -168,7 +168,6 @@ int dmm_paged_attention(const void *q, int64_t q_ld, int heads, float scale, voi
     p.q_ld = q_ld;
     p.out_ld = out_ld;
     p.group = heads / cache->kv_heads;
-    p.q_tiles = (p.group + 15) / 16;
     p.scale = scale;
     const bool pdl = (flags & DMM_FLAG_PDL) != 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,13 +1,15 @@
 // Attention of one new token per sequence over a paged cache.
 //
-// out = sum_j p_j v_j / sum_j p_j with p_j = exp2(c q . k_j - m), c = scale log2(e): every key and value is read once and used
+// out = sum_j p_j v_j / sum_j p_j with p_j = 2^(c q . k_j - m), c = scale log2(e): every key and value is read once and used
 // for the few query heads that share it, so the cache's bytes are the bound.
 //
-// The work is cut into units of 16 keys of one (sequence, key head), a segment being all units of one; the units of all
-// segments in one line are divided evenly, first among the CTAs, one per SM, then among a CTA's eight warps.  A
-// warp streams its units through a ring of its own in shared memory (cp.async, a page never ends inside a unit), and works
-// on warp-level tensor cores: S[16 queries, 16 keys] = Q K^T, P V with the fragments of S as operands.  With
-// group <= 8 half of the 16 rows is idle, which costs nothing: the multiplications take a fifth of the time of the bytes.
+// The work is cut into units of 16 keys of one (sequence, key head, tile of queries), a segment being all units of one; the
+// units of all segments in one line are divided evenly, first among the CTAs, one per SM, then among a CTA's eight
+// warps.  A warp streams its units through a ring of its own in shared memory (cp.async; a page never ends inside a unit) and
+// works on warp-level tensor cores with the keys as the 16 rows and 8 queries as the columns: S^T[16, 8] = K Q^T and
+// O^T[D, 8] += V^T P^T, where P^T is S^T transposed in registers.  (Queries as rows would leave half of them idle
+// and take twice the registers.)  Groups of more than 8 query heads have two such column tiles, of more than 16 several tiles
+// that read the keys again.
 // No barrier until a warp has finished.  A segment that a warp has whole is written out by it.  What several warps have of
 // one segment is joined through shared memory, what several CTAs have through the workspace by a second kernel: always in the
 // order of the keys, so that results do not depend on who comes first.
@@ -28,19 +30,20 @@ struct DecodeParams {
     float *partial;  // [2 * CTAs][16][D], then [2 * CTAs][16][2]: maximum and sum
     long long q_ld, out_ld;
     CacheView cache;
-    int group, q_tiles;  // q_tiles: of 16 query heads that share a key head
+    int group, q_tiles;  // q_tiles: of 8 kN query heads that share a key head
     float scale;
 };
 
-// A part of a segment: weighted sums of values (rows padded against bank conflicts), then maximum and sum of each row.
-template <int D, int kRows>
+// kN: column tiles of 8 queries.
+template <int D, int kN>
 struct DecodePlan {
-    static constexpr int kStages = (D == 128 ? 3 : 6) - (kRows == 2 ? D == 128 ? 1 : 2 : 0);
+    static constexpr int kStages = (D == 128 ? 3 : 6) - (kN == 2 ? D == 128 ? 1 : 2 : 0);
     static constexpr uint32_t kRowBytes = 2 * D;
     static constexpr uint32_t kUnitBytes = kUnitKeys * kRowBytes;  // of K, and again of V
     static constexpr uint32_t kWarpBytes = kStages * 2 * kUnitBytes;
-    static constexpr int kPad = D + 4;
-    static constexpr int kPartFloats = 8 * kRows * (kPad + 2);
+    // A part of a segment: weighted sums of values (a row per query, padded against bank conflicts), then maximum and sum of each.
+    static constexpr int kRows = 8 * kN, kPad = D + 4;
+    static constexpr int kPartFloats = kRows * (kPad + 2);
     // the rings, and a part per warp beside them; a warp's last part takes the place of its ring
     static constexpr uint32_t kParts = kDecodeWarps * kWarpBytes;
     static constexpr uint32_t kBytes = kParts + kDecodeWarps * kPartFloats * 4;
@@ -50,26 +53,43 @@ struct DecodePlan {
 
 inline size_t decode_workspace(int head_dim, int ctas) { return static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2) * sizeof(float); }
 
-// Where a unit lies: segment (seq, head, with head counting the tiles of 16 queries too), unit within it, and the segment's
-// length.  A sequence without keys has one unit, without keys.
-struct DecodeAt {
-    long long start;  // unit number of the segment's first
-    int seq, head, unit, units, len;
-};
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnitKeys - 1) / kUnitKeys : 1; }
 
-// Units of all sequences, and the place of unit `u` of them.  By the lanes of a warp.
-__device__ __forceinline__ long long decode_units(const CacheView &c, int heads) {
+// `all` units over `ctas` CTAs: CTA x has [begin(x), begin(x + 1)), the first `more` of them one unit more than the others.
+struct DecodeShare {
+    long long all, each;
+    int more;
+    __device__ __forceinline__ long long begin(int x) const { return each * x + min(x, more); }
+};
+// By the lanes of a warp.  A sequence without keys has one unit, without keys.
+__device__ __forceinline__ DecodeShare decode_share(const CacheView &c, int heads, int ctas) {
     const int lane = threadIdx.x & 31;
     long long sum = 0;
     for (int b = lane; b < c.num_seqs; b += 32) sum += units_of(cache_len(c, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum * heads;
+    DecodeShare s;
+    s.all = sum * heads;
+    if ((s.all >> 32) == 0) {  // (a division of 64 bits takes a microsecond)
+        const unsigned n = static_cast<unsigned>(s.all), d = n / static_cast<unsigned>(ctas);
+        s.each = d;
+        s.more = static_cast<int>(n - d * static_cast<unsigned>(ctas));
+    } else {
+        s.each = s.all / ctas;
+        s.more = static_cast<int>(s.all - s.each * ctas);
+    }
+    return s;
 }
-__device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int heads, long long u) {
-    const int lane = threadIdx.x & 31;
-    DecodeAt at = {0, 0, 0, 0, 1, 0};
+
+// Where a unit lies: the segment (sequence, key head, tile of its queries), its length, its first unit's number and the unit in it.
+struct DecodeAt {
+    long long start;
+    int seq, head, tile, unit, units, len;
+};
+// The place of unit u, by the lanes of a warp.
+__device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int q_tiles, long long u) {
+    const int lane = threadIdx.x & 31, heads = c.kv_heads * q_tiles;
+    DecodeAt at = {0, 0, 0, 0, 0, 1, 0};
     long long before = 0;
     for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
         const int b = b0 + lane, len = b < c.num_seqs ? cache_len(c, b) : 0;
@@ -86,9 +106,12 @@ __device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int heads, lon
             at.seq = b0 + who;
             at.len = __shfl_sync(0xffffffffu, len, who);
             at.units = units_of(at.len);
-            const long long first = before + __shfl_sync(0xffffffffu, upto - mine, who);
-            at.head = static_cast<int>((u - first) / at.units);
-            at.start = first + static_cast<long long>(at.head) * at.units;
+            const long long first = before + __shfl_sync(0xffffffffu, upto - mine, who), rest = u - first;
+            const int segment = (rest >> 32) == 0 ? static_cast<int>(static_cast<unsigned>(rest) / static_cast<unsigned>(at.units))
+                                                  : static_cast<int>(rest / at.units);
+            at.head = q_tiles == 1 ? segment : segment / q_tiles;
+            at.tile = segment - at.head * q_tiles;
+            at.start = first + static_cast<long long>(segment) * at.units;
             at.unit = static_cast<int>(u - at.start);
             return at;
         }
@@ -96,16 +119,20 @@ __device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int heads, lon
     }
     return at;
 }
-__device__ __forceinline__ void decode_next(const CacheView &c, int heads, DecodeAt &at) {
-    if (++at.unit < at.units) return;
+// The next unit; true when it is of another segment.
+__device__ __forceinline__ bool decode_next(const CacheView &c, int q_tiles, DecodeAt &at) {
+    if (++at.unit < at.units) return false;
     at.start += at.units;
     at.unit = 0;
-    if (++at.head < heads) return;
+    if (++at.tile < q_tiles) return true;
+    at.tile = 0;
+    if (++at.head < c.kv_heads) return true;
     at.head = 0;
     if (++at.seq < c.num_seqs) {
         at.len = cache_len(c, at.seq);
         at.units = units_of(at.len);
     }
+    return true;
 }
 
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool have) {
@@ -123,6 +150,12 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
                  : "r"(addr)
                  : "memory");
 }
+// An 8 x 8 tile of 16-bit values that a warp holds as a fragment, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t w) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
 template <class T>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -137,226 +170,225 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
 // What a warp has of one segment when it could not write it out.
 struct DecodePart {
     long long start;
-    int seq, head, units, have;  // have: units of it that this part covers, 0 = no part
+    int seq, head, tile, units, have;  // have: units of it that this part covers, 0 = no part
 };
 
-// kRows: 1 for groups of up to 8 query heads, 2 for up to 16 (rows lane / 4 and lane / 4 + 8 of a fragment)
-template <class T, int D, int kRows>
+template <class T, int D, int kN>
 __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(const DecodeParams p) {
-    using Plan = DecodePlan<D, kRows>;
+    using Plan = DecodePlan<D, kN>;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     __shared__ DecodePart s_part[2 * kDecodeWarps];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, pair = lane % 4;
-    const uint32_t smem = smem_u32(smem_raw);
     grid_dep_wait();
-    grid_dep_launch();  // the kernel that joins the CTAs' parts may take its place; it waits for this one's end
-    const int heads = p.cache.kv_heads * p.q_tiles;
-    const long long all = decode_units(p.cache, heads);
-    const long long c0 = part_begin(all, gridDim.x, blockIdx.x), c1 = part_begin(all, gridDim.x, blockIdx.x + 1);
-    const long long u0 = c0 + (c1 - c0) * warp / kDecodeWarps, u1 = c0 + (c1 - c0) * (warp + 1) / kDecodeWarps;
+    grid_dep_launch();  // the kernel that joins the CTAs' parts may come in beside this one; it waits for this one's end
+    const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, gridDim.x);
+    const long long c0 = share.begin(blockIdx.x);
+    const long long mine = share.begin(blockIdx.x + 1) - c0;
+    const long long u0 = c0 + mine * warp / kDecodeWarps, u1 = c0 + mine * (warp + 1) / kDecodeWarps;
     if (lane < 2) s_part[2 * warp + lane].have = 0;
     __syncwarp();
 
-    const uint32_t ring = smem + warp * Plan::kWarpBytes;
-    // pieces of 16 bytes: a row has D / 8 of them, piece c of row r lies at c ^ (r % 8), so that eight rows' same piece is conflict free
-    constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
-    const int piece = lane % kPieces, row0 = lane / kPieces;
-
-    float o[D / 8][4], m[2], l[2];
-    uint32_t qf[D / 16][4];
-    const float c = p.scale * 1.4426950408889634f;
-    float *const first_part = reinterpret_cast<float *>(smem_raw + Plan::kParts) + warp * Plan::kPartFloats;
-    float *const last_part = reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
-
-    DecodeAt load = {}, at = {};
-    int page = 0;
-    const auto fetch_page = [&](const DecodeAt &w) {
-        return w.len > 0 ? p.cache.page_table[w.seq * p.cache.table_stride + ((w.unit * kUnitKeys) >> p.cache.page_shift)] : -1;
-    };
-    const auto issue = [&](int stage) {
-        const int pos = load.unit * kUnitKeys, keys = load.len - pos;
-        bool there = keys > 0;
-        if (there && (page < 0 || page >= p.cache.num_pages)) {
-            raise_status(DMM_STATUS_BAD_PAGE);
-            there = false;
-        }
-        const long long base = there ? page * p.cache.page_stride + (load.head / p.q_tiles) * p.cache.head_stride +
-                                           (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride
-                                     : 0;
-        const T *k = static_cast<const T *>(p.cache.k) + base + piece * 8, *v = static_cast<const T *>(p.cache.v) + base + piece * 8;
-        const uint32_t dst = ring + stage * 2 * Plan::kUnitBytes;
-#pragma unroll
-        for (int r = row0; r < kUnitKeys; r += kRowsAtOnce) {
-            const bool have = there && r < keys;
-            const uint32_t d = dst + r * Plan::kRowBytes + ((piece ^ (r & 7)) << 4);
-            const long long off = have ? r * p.cache.row_stride : 0;
-            cp_async16_or_zero(d, k + off, have);
-            cp_async16_or_zero(d + Plan::kUnitBytes, v + off, have);
-        }
-    };
-
     if (u0 < u1) {
-        at = decode_at(p.cache, heads, u0);
-        load = at;
-        long long ahead = u0;  // the next unit to load
-        page = fetch_page(load);
+        const uint32_t ring = smem_u32(smem_raw) + warp * Plan::kWarpBytes;
+        // pieces of 16 bytes: a row has D / 8 of them, piece c of row r lies at c ^ (r % 8), so that eight rows' same piece is conflict free
+        constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;
+        const int piece = lane % kPieces, row0 = lane / kPieces;
+        const long long my_offset = row0 * p.cache.row_stride + piece * 8, step = kRowsAtOnce * p.cache.row_stride;
+        const float c = p.scale * 1.4426950408889634f;
+
+        DecodeAt at = decode_at(p.cache, p.q_tiles, u0), load = at;
+        int left = static_cast<int>(u1 - u0);  // units not yet asked for
+        const int32_t *table = p.cache.page_table + load.seq * p.cache.table_stride;
+        int page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
+        // asks for the unit at `load`, and goes on to the next, whose page number is then under way
+        const auto issue = [&](int stage) {
+            const int pos = load.unit * kUnitKeys, keys = load.len - pos;
+            const bool there = page >= 0 && page < p.cache.num_pages;
+            if (!there) raise_status(DMM_STATUS_BAD_PAGE);
+            const uint32_t dst = ring + stage * 2 * Plan::kUnitBytes + row0 * Plan::kRowBytes;
+            if (there && keys >= kUnitKeys) {
+                const long long base = page * p.cache.page_stride + load.head * p.cache.head_stride +
+                                       (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride + my_offset;
+                const T *k = static_cast<const T *>(p.cache.k) + base, *v = static_cast<const T *>(p.cache.v) + base;
 #pragma unroll
-        for (int s = 0; s < Plan::kStages - 1; ++s) {
-            if (ahead < u1) {
-                issue(s);
-                if (++ahead < u1) {
-                    decode_next(p.cache, heads, load);
-                    page = fetch_page(load);
+                for (int i = 0; i < kUnitKeys / kRowsAtOnce; ++i) {
+                    const uint32_t d = dst + i * kRowsAtOnce * Plan::kRowBytes + ((piece ^ ((row0 + i * kRowsAtOnce) & 7)) << 4);
+                    cp_async16(d, k);
+                    cp_async16(d + Plan::kUnitBytes, v);
+                    k += step;
+                    v += step;
+                }
+            } else {  // the sequence's last unit: what is behind its end becomes zeros
+                const long long base = there ? page * p.cache.page_stride + load.head * p.cache.head_stride +
+                                                   (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride
+                                             : 0;
+                const T *k = static_cast<const T *>(p.cache.k) + base, *v = static_cast<const T *>(p.cache.v) + base;
+#pragma unroll 1
+                for (int i = 0; i < kUnitKeys / kRowsAtOnce; ++i) {
+                    const int row = row0 + i * kRowsAtOnce;
+                    const bool have = there && row < keys;
+                    const uint32_t d = dst + i * kRowsAtOnce * Plan::kRowBytes + ((piece ^ (row & 7)) << 4);
+                    const long long off = have ? i * step + my_offset : 0;
+                    cp_async16_or_zero(d, k + off, have);
+                    cp_async16_or_zero(d + Plan::kUnitBytes, v + off, have);
                 }
             }
+            if (--left > 0) {
+                if (decode_next(p.cache, p.q_tiles, load)) table = p.cache.page_table + load.seq * p.cache.table_stride;
+                page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < Plan::kStages - 1; ++s) {
+            if (left > 0) issue(s);
             cp_async_commit();
         }
-        int stage = 0;
+
+        float o[kN][D / 16][4], m[kN][2], l[kN][2];
+        uint32_t qf[kN][D / 16][2];
+        int stage = 0, have = 0;
         bool fresh = true;
-        int have = 0;
-        for (long long u = u0; u < u1; ++u) {
+        const int a_row = ((lane / 8) % 2) * 8 + lane % 8, a_half = lane / 16;   // of K: (keys, 16-byte pieces) of the four tiles of a fragment
+        const int v_row = (lane / 16) * 8 + lane % 8, v_half = (lane / 8) % 2;   // of V, which is read transposed
+        for (int n = static_cast<int>(u1 - u0); n > 0; --n) {
             if (fresh) {
-                const T *q = static_cast<const T *>(p.q) + at.seq * p.q_ld + static_cast<long long>(at.head / p.q_tiles) * p.group * D;
-                const int r0 = (at.head % p.q_tiles) * 16 + quad;
+                const T *q = static_cast<const T *>(p.q) + at.seq * p.q_ld + static_cast<long long>(at.head) * p.group * D + 2 * pair;
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k)
+                for (int t = 0; t < kN; ++t) {
+                    const int r = at.tile * Plan::kRows + 8 * t + quad;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        qf[k][2 * h] = r0 < p.group ? *reinterpret_cast<const uint32_t *>(q + r0 * D + 16 * k + 8 * h + 2 * pair) : 0u;
-                        qf[k][2 * h + 1] = kRows == 2 && r0 + 8 < p.group ? *reinterpret_cast<const uint32_t *>(q + (r0 + 8) * D + 16 * k + 8 * h + 2 * pair) : 0u;
-                    }
+                    for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)
+                        for (int h = 0; h < 2; ++h) qf[t][k][h] = r < p.group ? *reinterpret_cast<const uint32_t *>(q + r * D + 16 * k + 8 * h) : 0u;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) o[n][x] = 0.0f;
-                m[0] = m[1] = -INFINITY;
-                l[0] = l[1] = 0.0f;
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[t][k][x] = 0.0f;
+                    m[t][0] = m[t][1] = -INFINITY;
+                    l[t][0] = l[t][1] = 0.0f;
+                }
                 fresh = false;
                 have = 0;
             }
             cp_async_wait<Plan::kStages - 2>();
             __syncwarp();  // all lanes' pieces of this unit are there, and all have read the unit before
-            if (ahead < u1) {
-                issue(stage == 0 ? Plan::kStages - 1 : stage - 1);
-                if (++ahead < u1) {
-                    decode_next(p.cache, heads, load);
-                    page = fetch_page(load);
-                }
-            }
+            if (left > 0) issue(stage == 0 ? Plan::kStages - 1 : stage - 1);
             cp_async_commit();
 
             const uint32_t kb = ring + stage * 2 * Plan::kUnitBytes, vb = kb + Plan::kUnitBytes;
-            float s[2][4] = {};
-            {
-                const int r = (lane / 16) * 8 + lane % 8, half = (lane / 8) % 2;
-                const uint32_t row = kb + r * Plan::kRowBytes;
+            float s[kN][2][4] = {};  // two chains of products, added at the end
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    uint32_t b[4];
-                    ldsm4(row + (((2 * k + half) ^ (r & 7)) << 4), b);
-                    mma16<T>(s[0], qf[k], b[0], b[1]);
-                    mma16<T>(s[1], qf[k], b[2], b[3]);
-                }
+            for (int k = 0; k < D / 16; ++k) {
+                uint32_t a[4];
+                ldsm4(kb + a_row * Plan::kRowBytes + (((2 * k + a_half) ^ (a_row & 7)) << 4), a);
+#pragma unroll
+                for (int t = 0; t < kN; ++t) mma16<T>(s[t][k & 1], a, qf[t][k][0], qf[t][k][1]);
             }
             const int keys = at.len - at.unit * kUnitKeys;
-            uint32_t pf[4] = {};
-            float top[kRows];
-#pragma unroll
-            for (int h = 0; h < kRows; ++h) {
-                top[h] = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float &v = s[n][2 * h + x];
-                        v = 8 * n + 2 * pair + x < keys ? v * c : -INFINITY;
-                        top[h] = fmaxf(top[h], v);
-                    }
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            }
+            float x[kN][4];  // keys quad and quad + 8 of queries 2 pair and 2 pair + 1
+            float top[kN][2];
             bool rise = false;
 #pragma unroll
-            for (int h = 0; h < kRows; ++h) rise |= top[h] > m[h] + 8.0f;
+            for (int t = 0; t < kN; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] = (s[t][0][i] + s[t][1][i]) * c;
+                    if (quad + 8 * (i / 2) >= keys) x[t][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    top[t][i] = fmaxf(x[t][i], x[t][i + 2]);
+                    top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 4));
+                    top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 8));
+                    top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 16));
+                    rise |= top[t][i] > m[t][i] + 8.0f;
+                }
+            }
             if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-                for (int h = 0; h < kRows; ++h) {
-                    const float to = fmaxf(m[h], top[h]), f = m[h] == -INFINITY ? 0.0f : exp2_fast(m[h] - to);
-                    m[h] = to;
-                    l[h] *= f;
+                for (int t = 0; t < kN; ++t)
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) {
-                        o[n][2 * h] *= f;
-                        o[n][2 * h + 1] *= f;
+                    for (int i = 0; i < 2; ++i) {
+                        const float to = fmaxf(m[t][i], top[t][i]), f = m[t][i] == -INFINITY ? 0.0f : exp2_fast(m[t][i] - to);
+                        m[t][i] = to;
+                        l[t][i] *= f;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            o[t][k][i] *= f;
+                            o[t][k][i + 2] *= f;
+                        }
                     }
+            }
+            uint32_t pf[kN][2];
+#pragma unroll
+            for (int t = 0; t < kN; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] = exp2_fast(x[t][i] - (m[t][i % 2] == -INFINITY ? 0.0f : m[t][i % 2]));
+                    l[t][i % 2] += x[t][i];
                 }
+                pf[t][0] = transposed(pack16<T>(x[t][0], x[t][1]));
+                pf[t][1] = transposed(pack16<T>(x[t][2], x[t][3]));
             }
 #pragma unroll
-            for (int h = 0; h < kRows; ++h) {
-                const float mm = m[h] == -INFINITY ? 0.0f : m[h];
+            for (int k = 0; k < D / 16; ++k) {
+                uint32_t a[4];
+                ldsm4_trans(vb + v_row * Plan::kRowBytes + (((2 * k + v_half) ^ (v_row & 7)) << 4), a);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float a = exp2_fast(s[n][2 * h] - mm), b = exp2_fast(s[n][2 * h + 1] - mm);
-                    l[h] += a + b;
-                    pf[2 * n + h] = pack16<T>(a, b);
-                }
-            }
-            {
-                const int r = ((lane / 8) % 2) * 8 + lane % 8, half = lane / 16;
-                const uint32_t row = vb + r * Plan::kRowBytes;
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) {
-                    uint32_t b[4];
-                    ldsm4_trans(row + (((2 * n + half) ^ (r & 7)) << 4), b);
-                    mma16<T>(o[2 * n], pf, b[0], b[1]);
-                    mma16<T>(o[2 * n + 1], pf, b[2], b[3]);
-                }
+                for (int t = 0; t < kN; ++t) mma16<T>(o[t][k], a, pf[t][0], pf[t][1]);
             }
             if (++stage == Plan::kStages) stage = 0;
             ++have;
 
-            if (at.unit + 1 == at.units || u + 1 == u1) {  // the end of the segment or of this warp's share
+            if (at.unit + 1 == at.units || n == 1) {  // the end of the segment or of this warp's share
+                float *part = n > 1 ? reinterpret_cast<float *>(smem_raw + Plan::kParts) + warp * Plan::kPartFloats
+                                    : reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
+                __syncwarp();  // (the last part lies where all lanes have read the last unit)
 #pragma unroll
-                for (int h = 0; h < kRows; ++h) {
-                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-                }
-                const int r0 = (at.head % p.q_tiles) * 16 + quad;
-                if (have == at.units) {
-                    T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + static_cast<long long>(at.head / p.q_tiles) * p.group * D;
+                for (int t = 0; t < kN; ++t) {
 #pragma unroll
-                    for (int h = 0; h < kRows; ++h) {
-                        if (r0 + 8 * h >= p.group) continue;
-                        const float inv = at.len > 0 ? 1.0f / l[h] : 0.0f;
-#pragma unroll
-                        for (int n = 0; n < D / 8; ++n)
-                            *reinterpret_cast<uint32_t *>(out + (r0 + 8 * h) * D + 8 * n + 2 * pair) = pack16<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+                    for (int i = 0; i < 2; ++i) {
+                        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 4);
+                        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 8);
+                        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 16);
                     }
-                } else {
-                    const int which = u + 1 < u1 ? 0 : 1;
-                    float *part = which == 0 ? first_part : last_part;
-                    __syncwarp();  // (the last part lies where all lanes have read the last unit)
+                    if (have == at.units) {
+                        const int r = at.tile * Plan::kRows + 8 * t + quad;
+                        T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head) * p.group + r) * D + 2 * pair;
+                        const float i0 = at.len > 0 ? 1.0f / l[t][0] : 0.0f, i1 = at.len > 0 ? 1.0f / l[t][1] : 0.0f;
 #pragma unroll
-                    for (int h = 0; h < kRows; ++h) {
-                        const int row = quad + 8 * h;
+                        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-                        for (int n = 0; n < D / 8; ++n)
-                            *reinterpret_cast<float2 *>(part + row * Plan::kPad + 8 * n + 2 * pair) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                        if (pair == 0) *reinterpret_cast<float2 *>(part + 8 * kRows * Plan::kPad + 2 * row) = make_float2(m[h], l[h]);
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t w = transposed(pack16<T>(o[t][k][2 * h] * i0, o[t][k][2 * h + 1] * i1));
+                                if (r < p.group) *reinterpret_cast<uint32_t *>(out + 16 * k + 8 * h) = w;
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int row = 8 * t + 2 * pair + i;
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                part[row * Plan::kPad + 16 * k + quad] = o[t][k][i];
+                                part[row * Plan::kPad + 16 * k + quad + 8] = o[t][k][i + 2];
+                            }
+                            if (quad == 0) *reinterpret_cast<float2 *>(part + Plan::kRows * Plan::kPad + 2 * row) = make_float2(m[t][i], l[t][i]);
+                        }
                     }
-                    if (lane == 0) s_part[2 * warp + which] = {at.start, at.seq, at.head, at.units, have};
                 }
+                if (have != at.units && lane == 0) s_part[2 * warp + (n > 1 ? 0 : 1)] = {at.start, at.seq, at.head, at.tile, at.units, have};
                 fresh = true;
             }
-            decode_next(p.cache, heads, at);
+            decode_next(p.cache, p.q_tiles, at);
         }
+        cp_async_wait<0>();
     }
-    cp_async_wait<0>();
     __syncthreads();
-    // Parts of one segment lie next to each other in the warps' order: a warp joins the parts of every eighth segment.
+    // Parts of one segment lie next to each other in the warps' order.  A warp takes every eighth row of what there is to join.
     int nth = 0;
     for (int i = 0; i < 2 * kDecodeWarps;) {
         if (s_part[i].have == 0) {
@@ -366,39 +398,45 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         const DecodePart of = s_part[i];
         int end = i + 1, have = of.have;
         while (end < 2 * kDecodeWarps && (s_part[end].have == 0 || s_part[end].start == of.start)) have += s_part[end++].have;
-        if (nth++ % kDecodeWarps == warp) {
+        const auto part_of = [&](int x) {
+            return x % 2 == 0 ? reinterpret_cast<const float *>(smem_raw + Plan::kParts) + x / 2 * Plan::kPartFloats
+                              : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
+        };
+        const int rows = min(Plan::kRows, p.group - of.tile * Plan::kRows);
+        for (int row = 0; row < rows; ++row) {
+            if (nth++ % kDecodeWarps != warp) continue;
             constexpr int kC = D / 32;  // columns of a lane
-            const auto part_of = [&](int x) {
-                return x % 2 == 0 ? reinterpret_cast<const float *>(smem_raw + Plan::kParts) + x / 2 * Plan::kPartFloats
-                                  : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
-            };
-            for (int row = 0; row < 8 * kRows; ++row) {
-                const int r = (of.head % p.q_tiles) * 16 + row;
-                if (r >= p.group) break;
-                float top = -INFINITY, sum = 0.0f, acc[kC] = {};
-                for (int x = i; x < end; ++x)
-                    if (s_part[x].have > 0) top = fmaxf(top, part_of(x)[8 * kRows * Plan::kPad + 2 * row]);
-                for (int x = i; x < end; ++x) {
-                    if (s_part[x].have == 0) continue;
-                    const float *part = part_of(x);
-                    const float mx = part[8 * kRows * Plan::kPad + 2 * row], w = mx == -INFINITY ? 0.0f : exp2_fast(mx - top);
-                    sum += w * part[8 * kRows * Plan::kPad + 2 * row + 1];
+            // lane x: maximum and sum of part x
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (lane >= i && lane < end && s_part[lane].have > 0) ml = *reinterpret_cast<const float2 *>(part_of(lane) + Plan::kRows * Plan::kPad + 2 * row);
+            float top = ml.x;
 #pragma unroll
-                    for (int y = 0; y < kC; ++y) acc[y] += w * part[row * Plan::kPad + kC * lane + y];
-                }
-                if (have == of.units) {
-                    T *out = static_cast<T *>(p.out) + of.seq * p.out_ld + (static_cast<long long>(of.head / p.q_tiles) * p.group + r) * D + kC * lane;
-                    const float inv = 1.0f / sum;
+            for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+            top = __shfl_sync(0xffffffffu, top, 0);
+            const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
+            float sum = w * ml.y, acc[kC] = {};
 #pragma unroll
-                    for (int y = 0; y < kC; y += 2) *reinterpret_cast<uint32_t *>(out + y) = pack16<T>(acc[y] * inv, acc[y + 1] * inv);
-                } else {  // a CTA has at most one segment that began before it, and one that goes on behind it
-                    const int slot = 2 * blockIdx.x + (of.start < c0 ? 0 : 1);
-                    float *to = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
+            for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            sum = __shfl_sync(0xffffffffu, sum, 0);
+            for (int x = i; x < end; ++x) {
+                const float wx = __shfl_sync(0xffffffffu, w, x);
+                if (s_part[x].have == 0) continue;
+                const float *part = part_of(x) + row * Plan::kPad + kC * lane;
 #pragma unroll
-                    for (int y = 0; y < kC; ++y) to[y] = acc[y];
-                    if (lane == 0)
-                        *reinterpret_cast<float2 *>(p.partial + static_cast<size_t>(gridDim.x) * 2 * 16 * D + 2 * (slot * 16 + row)) = make_float2(top, sum);
-                }
+                for (int y = 0; y < kC; ++y) acc[y] += wx * part[y];
+            }
+            if (have == of.units) {
+                T *out = static_cast<T *>(p.out) + of.seq * p.out_ld + (static_cast<long long>(of.head) * p.group + of.tile * Plan::kRows + row) * D + kC * lane;
+                const float inv = 1.0f / sum;
+#pragma unroll
+                for (int y = 0; y < kC; y += 2) *reinterpret_cast<uint32_t *>(out + y) = pack16<T>(acc[y] * inv, acc[y + 1] * inv);
+            } else {  // a CTA has at most one segment that began before it, and one that goes on behind it
+                const int slot = 2 * blockIdx.x + (of.start < c0 ? 0 : 1);
+                float *to = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
+#pragma unroll
+                for (int y = 0; y < kC; ++y) to[y] = acc[y];
+                if (lane == 0)
+                    *reinterpret_cast<float2 *>(p.partial + static_cast<size_t>(gridDim.x) * 2 * 16 * D + 2 * (slot * 16 + row)) = make_float2(top, sum);
             }
         }
         i = end;
@@ -407,56 +445,48 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
 
 // Joins what several CTAs have of one segment.  Block (x, row): the segment that crosses from CTA x to the next, if x is the first
 // CTA that has a part of it.  Warps take the parts in turn, in the order of the keys.
-template <class T, int D>
+template <class T, int D, int kN>
 __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const DecodeParams p, int ctas) {
-    __shared__ float s_w[1024], s_acc[kDecodeWarps][D], s_red[kDecodeWarps];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.y;
-    const int heads = p.cache.kv_heads * p.q_tiles;
-    // (lengths are older than the kernel in front, which has waited for them)
-    const long long all = decode_units(p.cache, heads);
-    const long long c0 = part_begin(all, ctas, blockIdx.x), c1 = part_begin(all, ctas, blockIdx.x + 1);
-    bool work = c0 < c1 && c1 < all;
+    constexpr int kC = D / 32, kRows = 8 * kN;
+    __shared__ float s_acc[kDecodeWarps][D];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.y, x0 = blockIdx.x;
+    // (the lengths are older than the kernel in front, which has waited for them)
+    const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, ctas);
+    const long long c0 = share.begin(x0), c1 = share.begin(x0 + 1);
+    bool work = c0 < c1 && c1 < share.all;
     DecodeAt at = {};
     int r = 0;
     if (work) {
-        at = decode_at(p.cache, heads, c1);
-        r = (at.head % p.q_tiles) * 16 + row;
+        at = decode_at(p.cache, p.q_tiles, c1);
+        r = at.tile * kRows + row;
         work = at.unit > 0 && at.start >= c0 && r < p.group;
     }
+    // (block 0 waits in any case: this kernel must not end before the one in front)
+    if (!work && (x0 > 0 || row > 0)) return;
     grid_dep_wait();
     if (!work) return;
-    const int last = static_cast<int>(part_owner(all, ctas, at.start + at.units - 1)), n = last - static_cast<int>(blockIdx.x) + 1;
+    int n = 1;  // CTAs that have a part
+    while (share.begin(x0 + n) < at.start + at.units) ++n;
     const float *ml = p.partial + static_cast<size_t>(ctas) * 2 * 16 * D;
-    const auto slot_of = [&](int x) { return 2 * (static_cast<int>(blockIdx.x) + x) + (at.start < part_begin(all, ctas, blockIdx.x + x) ? 0 : 1); };
-    const auto empty = [&](int x) { return part_begin(all, ctas, blockIdx.x + x) == part_begin(all, ctas, blockIdx.x + x + 1); };
+    const auto slot_of = [&](int x) { return 2 * (x0 + x) + (x == 0 ? 1 : 0); };  // the segment begins in the first
+    // every warp: maximum and sum over all parts
     float top = -INFINITY;
-    for (int x = threadIdx.x; x < n; x += 32 * kDecodeWarps)
-        if (!empty(x)) top = fmaxf(top, ml[2 * (slot_of(x) * 16 + row)]);
+    for (int x = lane; x < n; x += 32) top = fmaxf(top, ml[2 * (slot_of(x) * 16 + row)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_red[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) top = fmaxf(top, s_red[w]);
-    __syncthreads();
     float sum = 0.0f;
-    for (int x = threadIdx.x; x < n; x += 32 * kDecodeWarps) {
-        const float2 v = empty(x) ? make_float2(-INFINITY, 0.0f) : *reinterpret_cast<const float2 *>(ml + 2 * (slot_of(x) * 16 + row));
-        const float w = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - top);
-        s_w[x] = w;
-        sum += w * v.y;
+    for (int x = lane; x < n; x += 32) {
+        const float2 v = *reinterpret_cast<const float2 *>(ml + 2 * (slot_of(x) * 16 + row));
+        sum += v.x == -INFINITY ? 0.0f : exp2_fast(v.x - top) * v.y;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_red[warp] = sum;
-    __syncthreads();
-    constexpr int kC = D / 32;
     float acc[kC] = {};
 #pragma unroll 4
     for (int x = warp; x < n; x += kDecodeWarps) {
-        const float w = s_w[x];
-        if (empty(x)) continue;
-        const float *from = p.partial + (static_cast<size_t>(slot_of(x)) * 16 + row) * D + kC * lane;
+        const int slot = slot_of(x);
+        const float mx = ml[2 * (slot * 16 + row)], w = mx == -INFINITY ? 0.0f : exp2_fast(mx - top);
+        const float *from = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
 #pragma unroll
         for (int y = 0; y < kC; ++y) acc[y] += w * from[y];
     }
@@ -464,22 +494,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const Dec
     for (int y = 0; y < kC; ++y) s_acc[warp][kC * lane + y] = acc[y];
     __syncthreads();
     if (threadIdx.x < D / 2) {
-        float a = 0.0f, b = 0.0f, all_sum = 0.0f;
+        float a = 0.0f, b = 0.0f;
 #pragma unroll
         for (int w = 0; w < kDecodeWarps; ++w) {
             a += s_acc[w][2 * threadIdx.x];
             b += s_acc[w][2 * threadIdx.x + 1];
-            all_sum += s_red[w];
         }
-        T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head / p.q_tiles) * p.group + r) * D;
-        *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack16<T>(a / all_sum, b / all_sum);
+        T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head) * p.group + r) * D;
+        *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack16<T>(a / sum, b / sum);
     }
 }
 
-template <class T, int D, int kRows>
-inline int launch_decode_typed(const DecodeParams &p, int ctas, bool pdl, cudaStream_t stream) {
-    using Plan = DecodePlan<D, kRows>;
-    const auto kernel = paged_attention_kernel<T, D, kRows>;
+template <class T, int D, int kN>
+inline int launch_decode_typed(DecodeParams &p, int ctas, bool pdl, cudaStream_t stream) {
+    using Plan = DecodePlan<D, kN>;
+    p.q_tiles = (p.group + Plan::kRows - 1) / Plan::kRows;
+    const auto kernel = paged_attention_kernel<T, D, kN>;
     static SmemAllowance allowance;
     const int rc = allowance.get(reinterpret_cast<const void *>(kernel), Plan::kBytes);
     if (rc) return rc;
@@ -495,14 +525,14 @@ inline int launch_decode_typed(const DecodeParams &p, int ctas, bool pdl, cudaSt
     cfg.numAttrs = pdl ? 1 : 0;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
     if (err != cudaSuccess) return err;
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(p.group < 16 ? p.group : 16));
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.group < Plan::kRows ? p.group : Plan::kRows));
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, p, ctas);
+    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, kN>, p, ctas);
 }
 
 template <class T, int D>
-inline int launch_decode(const DecodeParams &p, int ctas, bool pdl, cudaStream_t stream) {
+inline int launch_decode(DecodeParams &p, int ctas, bool pdl, cudaStream_t stream) {
     return p.group <= 8 ? launch_decode_typed<T, D, 1>(p, ctas, pdl, stream) : launch_decode_typed<T, D, 2>(p, ctas, pdl, stream);
 }
 
