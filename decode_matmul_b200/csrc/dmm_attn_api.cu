@@ -39,7 +39,7 @@ static int cache_view(const dmm_paged_cache *c, CacheView *view) {
         c->num_pages > 0x7fffffff || c->table_stride < c->max_pages)
         return DMM_ERR_SHAPE;
     // positions are 32-bit numbers
-    if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fff0000ll) return DMM_ERR_SHAPE;
+    if (static_cast<long long>(c->max_pages) * c->page_size > (1ll << 30)) return DMM_ERR_SHAPE;
     if (!aligned16(c->k) || !aligned16(c->v)) return DMM_ERR_ALIGN;
     // no two rows overlap: from the smallest stride on, each holds all of the one before
     struct {

@@ -44,14 +44,20 @@ struct DecodePlan {
     // A part of a segment: weighted sums of values (a row per query, padded against bank conflicts), then maximum and sum of each.
     static constexpr int kRows = 8 * kN, kPad = D + 4;
     static constexpr int kPartFloats = kRows * (kPad + 2);
-    // the rings, and a part per warp beside them; a warp's last part takes the place of its ring
-    static constexpr uint32_t kParts = kDecodeWarps * kWarpBytes;
-    static constexpr uint32_t kBytes = kParts + kDecodeWarps * kPartFloats * 4;
+    // the rings, and the queries of two segments per warp beside them; a warp's last part takes the place of its ring
+    static constexpr uint32_t kQBytes = kRows * kRowBytes;
+    static constexpr uint32_t kQ = kDecodeWarps * kWarpBytes;
+    static constexpr uint32_t kBytes = kQ + kDecodeWarps * 2 * kQBytes;
     static_assert(kPartFloats * 4 <= kWarpBytes, "a part fits into a ring");
     static_assert(kBytes <= 227 * 1024 - 1024, "shared memory");
 };
 
-inline size_t decode_workspace(int head_dim, int ctas) { return static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2) * sizeof(float); }
+// Workspace: what CTAs have of segments that they share, [2 * CTAs][16][D] and [2 * CTAs][16][2] floats, and behind it what a warp
+// has of the segment that began before its share, for the time until its CTA joins it.
+inline __host__ __device__ size_t decode_shared_floats(int head_dim, int ctas) { return static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2); }
+inline size_t decode_workspace(int head_dim, int ctas) {
+    return (decode_shared_floats(head_dim, ctas) + static_cast<size_t>(ctas) * kDecodeWarps * 16 * (head_dim + 6)) * sizeof(float);
+}
 
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnitKeys - 1) / kUnitKeys : 1; }
 
@@ -60,24 +66,26 @@ struct DecodeShare {
     long long all, each;
     int more;
     __device__ __forceinline__ long long begin(int x) const { return each * x + min(x, more); }
+    __device__ __forceinline__ int owner(long long u) const;
 };
-// By the lanes of a warp.  A sequence without keys has one unit, without keys.
+// a / b for numbers that nearly always fit into 32 bits (a division of 64 bits takes half a microsecond)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+    return a / b;
+}
+__device__ __forceinline__ int DecodeShare::owner(long long u) const {
+    const long long big = (each + 1) * more;
+    return static_cast<int>(u < big ? quotient(u, each + 1) : more + quotient(u - big, each));
+}
+// By the lanes of a warp.  A sequence without keys has one unit, without keys.  (32 sequences have less than 2^32 units.)
 __device__ __forceinline__ DecodeShare decode_share(const CacheView &c, int heads, int ctas) {
     const int lane = threadIdx.x & 31;
     long long sum = 0;
-    for (int b = lane; b < c.num_seqs; b += 32) sum += units_of(cache_len(c, b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int b0 = 0; b0 < c.num_seqs; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < c.num_seqs ? static_cast<unsigned>(units_of(cache_len(c, b0 + lane))) : 0u);
     DecodeShare s;
     s.all = sum * heads;
-    if ((s.all >> 32) == 0) {  // (a division of 64 bits takes a microsecond)
-        const unsigned n = static_cast<unsigned>(s.all), d = n / static_cast<unsigned>(ctas);
-        s.each = d;
-        s.more = static_cast<int>(n - d * static_cast<unsigned>(ctas));
-    } else {
-        s.each = s.all / ctas;
-        s.more = static_cast<int>(s.all - s.each * ctas);
-    }
+    s.each = quotient(s.all, ctas);
+    s.more = static_cast<int>(s.all - s.each * ctas);
     return s;
 }
 
@@ -93,29 +101,28 @@ __device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int q_tiles, l
     long long before = 0;
     for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
         const int b = b0 + lane, len = b < c.num_seqs ? cache_len(c, b) : 0;
-        const long long mine = b < c.num_seqs ? static_cast<long long>(units_of(len)) * heads : 0;
-        long long upto = mine;
+        const unsigned mine = b < c.num_seqs ? static_cast<unsigned>(units_of(len)) : 0u;
+        unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        const unsigned after = __ballot_sync(0xffffffffu, before + upto > u);
+        const unsigned after = __ballot_sync(0xffffffffu, before + static_cast<long long>(upto) * heads > u);
         if (after != 0) {
             const int who = __ffs(after) - 1;
             at.seq = b0 + who;
             at.len = __shfl_sync(0xffffffffu, len, who);
             at.units = units_of(at.len);
-            const long long first = before + __shfl_sync(0xffffffffu, upto - mine, who), rest = u - first;
-            const int segment = (rest >> 32) == 0 ? static_cast<int>(static_cast<unsigned>(rest) / static_cast<unsigned>(at.units))
-                                                  : static_cast<int>(rest / at.units);
+            const long long first = before + static_cast<long long>(__shfl_sync(0xffffffffu, upto - mine, who)) * heads;
+            const int segment = static_cast<int>(quotient(u - first, at.units));
             at.head = q_tiles == 1 ? segment : segment / q_tiles;
             at.tile = segment - at.head * q_tiles;
             at.start = first + static_cast<long long>(segment) * at.units;
             at.unit = static_cast<int>(u - at.start);
             return at;
         }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        before += static_cast<long long>(__shfl_sync(0xffffffffu, upto, 31)) * heads;
     }
     return at;
 }
@@ -188,7 +195,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
     const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, gridDim.x);
     const long long c0 = share.begin(blockIdx.x);
     const long long mine = share.begin(blockIdx.x + 1) - c0;
-    const long long u0 = c0 + mine * warp / kDecodeWarps, u1 = c0 + mine * (warp + 1) / kDecodeWarps;
+    const long long u0 = c0 + mine * warp / kDecodeWarps, u1 = c0 + mine * (warp + 1) / kDecodeWarps;  // (a power of two)
+    // what this warp has of a segment that began before its share and ends within it
+    float *const first_parts = p.partial + decode_shared_floats(D, gridDim.x) + static_cast<size_t>(blockIdx.x) * kDecodeWarps * Plan::kPartFloats;
     if (lane < 2) s_part[2 * warp + lane].have = 0;
     __syncwarp();
 
@@ -204,8 +213,27 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         int left = static_cast<int>(u1 - u0);  // units not yet asked for
         const int32_t *table = p.cache.page_table + load.seq * p.cache.table_stride;
         int page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
+        // The queries of a segment come with its first unit here, into one of two places in turn: at most two segments' are
+        // under way, since those of the present one are in registers by then.
+        const uint32_t q_place = smem_u32(smem_raw) + Plan::kQ + warp * 2 * Plan::kQBytes;
+        int q_load = 0, q_use = 0;
+        const auto issue_q = [&]() {
+            const int r0 = load.tile * Plan::kRows;
+            const T *q = static_cast<const T *>(p.q) + load.seq * p.q_ld + (static_cast<long long>(load.head) * p.group + r0) * D + piece * 8;
+            const uint32_t dst = q_place + q_load * Plan::kQBytes;
+            q_load ^= 1;
+#pragma unroll
+            for (int i = 0; i < Plan::kRows / kRowsAtOnce; ++i) {
+                const int row = row0 + i * kRowsAtOnce;
+                const bool have = r0 + row < p.group;
+                cp_async16_or_zero(dst + row * Plan::kRowBytes + ((piece ^ (row & 7)) << 4), have ? q + row * D : q, have);
+            }
+        };
+        issue_q();
         // asks for the unit at `load`, and goes on to the next, whose page number is then under way
+        bool fresh_load = false;
         const auto issue = [&](int stage) {
+            if (fresh_load) issue_q();
             const int pos = load.unit * kUnitKeys, keys = load.len - pos;
             const bool there = page >= 0 && page < p.cache.num_pages;
             if (!there) raise_status(DMM_STATUS_BAD_PAGE);
@@ -238,7 +266,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 }
             }
             if (--left > 0) {
-                if (decode_next(p.cache, p.q_tiles, load)) table = p.cache.page_table + load.seq * p.cache.table_stride;
+                fresh_load = decode_next(p.cache, p.q_tiles, load);
+                if (fresh_load) table = p.cache.page_table + load.seq * p.cache.table_stride;
                 page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
             }
         };
@@ -255,15 +284,20 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         const int a_row = ((lane / 8) % 2) * 8 + lane % 8, a_half = lane / 16;   // of K: (keys, 16-byte pieces) of the four tiles of a fragment
         const int v_row = (lane / 16) * 8 + lane % 8, v_half = (lane / 8) % 2;   // of V, which is read transposed
         for (int n = static_cast<int>(u1 - u0); n > 0; --n) {
+            cp_async_wait<Plan::kStages - 2>();
+            __syncwarp();  // all lanes' pieces of this unit are there, and all have read the unit before
             if (fresh) {
-                const T *q = static_cast<const T *>(p.q) + at.seq * p.q_ld + static_cast<long long>(at.head) * p.group * D + 2 * pair;
+                const uint32_t q = q_place + q_use * Plan::kQBytes;
+                q_use ^= 1;
 #pragma unroll
                 for (int t = 0; t < kN; ++t) {
-                    const int r = at.tile * Plan::kRows + 8 * t + quad;
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) qf[t][k][h] = r < p.group ? *reinterpret_cast<const uint32_t *>(q + r * D + 16 * k + 8 * h) : 0u;
+                    for (int k = 0; k < D / 32; ++k) {
+                        const int row = 8 * t + lane % 8;
+                        uint32_t b[4];
+                        ldsm4(q + row * Plan::kRowBytes + (((4 * k + lane / 8) ^ (row & 7)) << 4), b);
+                        qf[t][2 * k][0] = b[0], qf[t][2 * k][1] = b[1], qf[t][2 * k + 1][0] = b[2], qf[t][2 * k + 1][1] = b[3];
+                    }
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -273,9 +307,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 }
                 fresh = false;
                 have = 0;
+                __syncwarp();  // (the next queries but one come to this place)
             }
-            cp_async_wait<Plan::kStages - 2>();
-            __syncwarp();  // all lanes' pieces of this unit are there, and all have read the unit before
             if (left > 0) issue(stage == 0 ? Plan::kStages - 1 : stage - 1);
             cp_async_commit();
 
@@ -345,8 +378,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             ++have;
 
             if (at.unit + 1 == at.units || n == 1) {  // the end of the segment or of this warp's share
-                float *part = n > 1 ? reinterpret_cast<float *>(smem_raw + Plan::kParts) + warp * Plan::kPartFloats
-                                    : reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
+                float *part = n > 1 ? first_parts + warp * Plan::kPartFloats : reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
                 __syncwarp();  // (the last part lies where all lanes have read the last unit)
 #pragma unroll
                 for (int t = 0; t < kN; ++t) {
@@ -399,7 +431,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         int end = i + 1, have = of.have;
         while (end < 2 * kDecodeWarps && (s_part[end].have == 0 || s_part[end].start == of.start)) have += s_part[end++].have;
         const auto part_of = [&](int x) {
-            return x % 2 == 0 ? reinterpret_cast<const float *>(smem_raw + Plan::kParts) + x / 2 * Plan::kPartFloats
+            return x % 2 == 0 ? static_cast<const float *>(first_parts) + x / 2 * Plan::kPartFloats
                               : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
         };
         const int rows = min(Plan::kRows, p.group - of.tile * Plan::kRows);
@@ -449,6 +481,7 @@ template <class T, int D, int kN>
 __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const DecodeParams p, int ctas) {
     constexpr int kC = D / 32, kRows = 8 * kN;
     __shared__ float s_acc[kDecodeWarps][D];
+    __shared__ float2 s_ml[kDecodeWarps];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.y, x0 = blockIdx.x;
     // (the lengths are older than the kernel in front, which has waited for them)
     const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, ctas);
@@ -465,40 +498,65 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const Dec
     if (!work && (x0 > 0 || row > 0)) return;
     grid_dep_wait();
     if (!work) return;
-    int n = 1;  // CTAs that have a part
-    while (share.begin(x0 + n) < at.start + at.units) ++n;
+    const int n = share.owner(at.start + at.units - 1) - x0 + 1;  // CTAs that have a part
     const float *ml = p.partial + static_cast<size_t>(ctas) * 2 * 16 * D;
     const auto slot_of = [&](int x) { return 2 * (x0 + x) + (x == 0 ? 1 : 0); };  // the segment begins in the first
-    // every warp: maximum and sum over all parts
-    float top = -INFINITY;
-    for (int x = lane; x < n; x += 32) top = fmaxf(top, ml[2 * (slot_of(x) * 16 + row)]);
+    // the warp's own parts, eight at a time, with a maximum of its own: the loads wait for nothing but this kernel's start
+    constexpr int kAtOnce = 8;
+    float top = -INFINITY, sum = 0.0f, acc[kC] = {};
+    for (int x = warp; x < n; x += kDecodeWarps * kAtOnce) {
+        float2 v[kAtOnce];
+        float from[kAtOnce][kC];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f;
-    for (int x = lane; x < n; x += 32) {
-        const float2 v = *reinterpret_cast<const float2 *>(ml + 2 * (slot_of(x) * 16 + row));
-        sum += v.x == -INFINITY ? 0.0f : exp2_fast(v.x - top) * v.y;
-    }
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int xi = x + i * kDecodeWarps, slot = slot_of(xi);
+            v[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    float acc[kC] = {};
-#pragma unroll 4
-    for (int x = warp; x < n; x += kDecodeWarps) {
-        const int slot = slot_of(x);
-        const float mx = ml[2 * (slot * 16 + row)], w = mx == -INFINITY ? 0.0f : exp2_fast(mx - top);
-        const float *from = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
+            for (int y = 0; y < kC; ++y) from[i][y] = 0.0f;
+            if (xi < n) {
+                v[i] = *reinterpret_cast<const float2 *>(ml + 2 * (slot * 16 + row));
+                const float *src = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
+                if constexpr (kC == 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(src);
+                    from[i][0] = f.x, from[i][1] = f.y, from[i][2] = f.z, from[i][3] = f.w;
+                } else {
+                    const float2 f = *reinterpret_cast<const float2 *>(src);
+                    from[i][0] = f.x, from[i][1] = f.y;
+                }
+            }
+        }
+        float to = top;
 #pragma unroll
-        for (int y = 0; y < kC; ++y) acc[y] += w * from[y];
+        for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, v[i].x);
+        const float f = top == -INFINITY ? 0.0f : exp2_fast(top - to);
+        top = to;
+        sum *= f;
+#pragma unroll
+        for (int y = 0; y < kC; ++y) acc[y] *= f;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const float w = v[i].x == -INFINITY ? 0.0f : exp2_fast(v[i].x - top);
+            sum += w * v[i].y;
+#pragma unroll
+            for (int y = 0; y < kC; ++y) acc[y] += w * from[i][y];
+        }
     }
 #pragma unroll
     for (int y = 0; y < kC; ++y) s_acc[warp][kC * lane + y] = acc[y];
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
     __syncthreads();
     if (threadIdx.x < D / 2) {
-        float a = 0.0f, b = 0.0f;
+        float a = 0.0f, b = 0.0f, all = -INFINITY;
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; ++w) all = fmaxf(all, s_ml[w].x);
 #pragma unroll
         for (int w = 0; w < kDecodeWarps; ++w) {
-            a += s_acc[w][2 * threadIdx.x];
-            b += s_acc[w][2 * threadIdx.x + 1];
+            const float2 v = s_ml[w];
+            const float f = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - all);
+            sum += f * v.y;
+            a += f * s_acc[w][2 * threadIdx.x];
+            b += f * s_acc[w][2 * threadIdx.x + 1];
         }
         T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head) * p.group + r) * D;
         *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack16<T>(a / sum, b / sum);
