@@ -52,11 +52,11 @@ struct DecodePlan {
     static_assert(kBytes <= 227 * 1024 - 1024, "shared memory");
 };
 
-// Workspace: what CTAs have of segments that they share, [2 * CTAs][16][D] and [2 * CTAs][16][2] floats, and behind it what a warp
-// has of the segment that began before its share, for the time until its CTA joins it.
+// Workspace: what CTAs have of segments that they share, [2 * CTAs][16][D] and [2 * CTAs][16][2] floats, one description of such a
+// segment per CTA, and behind it what a warp has of the segment that began before its share, until its CTA joins it.
 inline __host__ __device__ size_t decode_shared_floats(int head_dim, int ctas) { return static_cast<size_t>(ctas) * 2 * 16 * (head_dim + 2); }
 inline size_t decode_workspace(int head_dim, int ctas) {
-    return (decode_shared_floats(head_dim, ctas) + static_cast<size_t>(ctas) * kDecodeWarps * 16 * (head_dim + 6)) * sizeof(float);
+    return (decode_shared_floats(head_dim, ctas) + static_cast<size_t>(ctas) * (4 + kDecodeWarps * 16 * (head_dim + 6))) * sizeof(float);
 }
 
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnitKeys - 1) / kUnitKeys : 1; }
@@ -77,44 +77,53 @@ __device__ __forceinline__ int DecodeShare::owner(long long u) const {
     const long long big = (each + 1) * more;
     return static_cast<int>(u < big ? quotient(u, each + 1) : more + quotient(u - big, each));
 }
-// By the lanes of a warp.  A sequence without keys has one unit, without keys.  (32 sequences have less than 2^32 units.)
-__device__ __forceinline__ DecodeShare decode_share(const CacheView &c, int heads, int ctas) {
-    const int lane = threadIdx.x & 31;
-    long long sum = 0;
-    for (int b0 = 0; b0 < c.num_seqs; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < c.num_seqs ? static_cast<unsigned>(units_of(cache_len(c, b0 + lane))) : 0u);
+// Where a unit lies: the segment (sequence, key head, tile of its queries), its length, its first unit's number and the unit in it.
+struct DecodeAt {
+    long long start;
+    int seq, head, tile, unit, units, len;
+};
+
+// Lengths and units of 32 sequences from b0 on, one per lane, and the running sum of the units.  A sequence without keys has one unit,
+// without keys; 32 sequences have less than 2^32.
+struct DecodeLens {
+    int len;
+    unsigned mine, upto;
+    __device__ __forceinline__ DecodeLens(const CacheView &c, int b0) {
+        const int lane = threadIdx.x & 31, b = b0 + lane;
+        len = b < c.num_seqs ? cache_len(c, b) : 0;
+        mine = b < c.num_seqs ? static_cast<unsigned>(units_of(len)) : 0u;
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+    }
+    __device__ __forceinline__ unsigned sum() const { return __shfl_sync(0xffffffffu, upto, 31); }
+};
+// All by the lanes of a warp; `first` are the lengths from sequence 0 on.
+__device__ __forceinline__ DecodeShare decode_share(const CacheView &c, const DecodeLens &first, int heads, int ctas) {
+    long long sum = first.sum();
+    for (int b0 = 32; b0 < c.num_seqs; b0 += 32) sum += DecodeLens(c, b0).sum();
     DecodeShare s;
     s.all = sum * heads;
     s.each = quotient(s.all, ctas);
     s.more = static_cast<int>(s.all - s.each * ctas);
     return s;
 }
-
-// Where a unit lies: the segment (sequence, key head, tile of its queries), its length, its first unit's number and the unit in it.
-struct DecodeAt {
-    long long start;
-    int seq, head, tile, unit, units, len;
-};
-// The place of unit u, by the lanes of a warp.
-__device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int q_tiles, long long u) {
-    const int lane = threadIdx.x & 31, heads = c.kv_heads * q_tiles;
+// The place of unit u.
+__device__ __forceinline__ DecodeAt decode_at(const CacheView &c, DecodeLens lens, int q_tiles, long long u) {
+    const int heads = c.kv_heads * q_tiles;
     DecodeAt at = {0, 0, 0, 0, 0, 1, 0};
     long long before = 0;
-    for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
-        const int b = b0 + lane, len = b < c.num_seqs ? cache_len(c, b) : 0;
-        const unsigned mine = b < c.num_seqs ? static_cast<unsigned>(units_of(len)) : 0u;
-        unsigned upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned after = __ballot_sync(0xffffffffu, before + static_cast<long long>(upto) * heads > u);
+    for (int b0 = 0;;) {
+        const unsigned after = __ballot_sync(0xffffffffu, before + static_cast<long long>(lens.upto) * heads > u);
         if (after != 0) {
             const int who = __ffs(after) - 1;
             at.seq = b0 + who;
-            at.len = __shfl_sync(0xffffffffu, len, who);
+            at.len = __shfl_sync(0xffffffffu, lens.len, who);
             at.units = units_of(at.len);
-            const long long first = before + static_cast<long long>(__shfl_sync(0xffffffffu, upto - mine, who)) * heads;
+            const long long first = before + static_cast<long long>(__shfl_sync(0xffffffffu, lens.upto - lens.mine, who)) * heads;
             const int segment = static_cast<int>(quotient(u - first, at.units));
             at.head = q_tiles == 1 ? segment : segment / q_tiles;
             at.tile = segment - at.head * q_tiles;
@@ -122,9 +131,11 @@ __device__ __forceinline__ DecodeAt decode_at(const CacheView &c, int q_tiles, l
             at.unit = static_cast<int>(u - at.start);
             return at;
         }
-        before += static_cast<long long>(__shfl_sync(0xffffffffu, upto, 31)) * heads;
+        before += static_cast<long long>(lens.sum()) * heads;
+        b0 += 32;
+        if (b0 >= c.num_seqs) return at;
+        lens = DecodeLens(c, b0);
     }
-    return at;
 }
 // The next unit; true when it is of another segment.
 __device__ __forceinline__ bool decode_next(const CacheView &c, int q_tiles, DecodeAt &at) {
@@ -183,6 +194,13 @@ struct DecodePart {
     long long start;
     int seq, head, tile, units, have;  // have: units of it that this part covers, 0 = no part
 };
+// The segment that begins in a CTA and goes on in others: what the join needs to know.
+struct DecodeCrossing {
+    int seq, head, tile, ctas;  // ctas: how many have a part of it, 0 = there is no such segment
+};
+__device__ __forceinline__ DecodeCrossing *decode_crossings(float *partial, int head_dim, int ctas) {
+    return reinterpret_cast<DecodeCrossing *>(partial + decode_shared_floats(head_dim, ctas));
+}
 
 template <class T, int D, int kN>
 __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(const DecodeParams p) {
@@ -192,12 +210,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, pair = lane % 4;
     grid_dep_wait();
     grid_dep_launch();  // the kernel that joins the CTAs' parts may come in beside this one; it waits for this one's end
-    const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, gridDim.x);
+    const DecodeLens lens(p.cache, 0);
+    const DecodeShare share = decode_share(p.cache, lens, p.cache.kv_heads * p.q_tiles, gridDim.x);
     const long long c0 = share.begin(blockIdx.x);
     const long long mine = share.begin(blockIdx.x + 1) - c0;
     const long long u0 = c0 + mine * warp / kDecodeWarps, u1 = c0 + mine * (warp + 1) / kDecodeWarps;  // (a power of two)
     // what this warp has of a segment that began before its share and ends within it
-    float *const first_parts = p.partial + decode_shared_floats(D, gridDim.x) + static_cast<size_t>(blockIdx.x) * kDecodeWarps * Plan::kPartFloats;
+    float *const first_parts = p.partial + decode_shared_floats(D, gridDim.x) + 4 * gridDim.x + static_cast<size_t>(blockIdx.x) * kDecodeWarps * Plan::kPartFloats;
     if (lane < 2) s_part[2 * warp + lane].have = 0;
     __syncwarp();
 
@@ -209,7 +228,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         const long long my_offset = row0 * p.cache.row_stride + piece * 8, step = kRowsAtOnce * p.cache.row_stride;
         const float c = p.scale * 1.4426950408889634f;
 
-        DecodeAt at = decode_at(p.cache, p.q_tiles, u0), load = at;
+        DecodeAt at = decode_at(p.cache, lens, p.q_tiles, u0), load = at;
         int left = static_cast<int>(u1 - u0);  // units not yet asked for
         const int32_t *table = p.cache.page_table + load.seq * p.cache.table_stride;
         int page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
@@ -420,59 +439,72 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         cp_async_wait<0>();
     }
     __syncthreads();
-    // Parts of one segment lie next to each other in the warps' order.  A warp takes every eighth row of what there is to join.
+    // Parts of one segment lie next to each other in the warps' order, first parts at even places; lane x looks at part x.  The
+    // warps take the rows of what there is to join in turn.
+    const int have = lane < 2 * kDecodeWarps ? s_part[lane].have : 0;
+    const long long start = lane < 2 * kDecodeWarps ? s_part[lane].start : 0;
+    const unsigned valid = __ballot_sync(0xffffffffu, have > 0), below = valid & ((1u << lane) - 1u);
+    const long long start_before = __shfl_sync(0xffffffffu, start, below != 0 ? 31 - __clz(below) : 0);
+    unsigned leaders = __ballot_sync(0xffffffffu, have > 0 && (below == 0 || start_before != start));
+    const float *const my_part = lane % 2 == 0 ? first_parts + lane / 2 * Plan::kPartFloats
+                                               : reinterpret_cast<const float *>(smem_raw + (lane / 2 % kDecodeWarps) * Plan::kWarpBytes);
+    DecodeCrossing crossing = {0, 0, 0, 0};
     int nth = 0;
-    for (int i = 0; i < 2 * kDecodeWarps;) {
-        if (s_part[i].have == 0) {
-            ++i;
-            continue;
-        }
+    while (leaders != 0) {
+        const int i = __ffs(leaders) - 1;
+        leaders &= leaders - 1;
+        const unsigned members = valid & (~0u << i) & (leaders != 0 ? (1u << (__ffs(leaders) - 1)) - 1u : ~0u);
+        const bool member = (members >> lane) & 1u;
         const DecodePart of = s_part[i];
-        int end = i + 1, have = of.have;
-        while (end < 2 * kDecodeWarps && (s_part[end].have == 0 || s_part[end].start == of.start)) have += s_part[end++].have;
-        const auto part_of = [&](int x) {
-            return x % 2 == 0 ? static_cast<const float *>(first_parts) + x / 2 * Plan::kPartFloats
-                              : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
-        };
+        const bool whole = __reduce_add_sync(0xffffffffu, member ? have : 0) == of.units;
+        const int slot = of.start < c0 ? 0 : 1;  // a CTA has at most one segment that began before it, and one that goes on behind it
+        if (!whole && slot == 1) crossing = {of.seq, of.head, of.tile, share.owner(of.start + of.units - 1) - static_cast<int>(blockIdx.x) + 1};
         const int rows = min(Plan::kRows, p.group - of.tile * Plan::kRows);
-        for (int row = 0; row < rows; ++row) {
-            if (nth++ % kDecodeWarps != warp) continue;
+        for (int row = (warp - nth) & (kDecodeWarps - 1); row < rows; row += kDecodeWarps) {
             constexpr int kC = D / 32;  // columns of a lane
-            // lane x: maximum and sum of part x
-            float2 ml = make_float2(-INFINITY, 0.0f);
-            if (lane >= i && lane < end && s_part[lane].have > 0) ml = *reinterpret_cast<const float2 *>(part_of(lane) + Plan::kRows * Plan::kPad + 2 * row);
+            const float2 ml = member ? *reinterpret_cast<const float2 *>(my_part + Plan::kRows * Plan::kPad + 2 * row) : make_float2(-INFINITY, 0.0f);
             float top = ml.x;
 #pragma unroll
-            for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-            top = __shfl_sync(0xffffffffu, top, 0);
+            for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
             const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
             float sum = w * ml.y, acc[kC] = {};
 #pragma unroll
-            for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            sum = __shfl_sync(0xffffffffu, sum, 0);
-            for (int x = i; x < end; ++x) {
-                const float wx = __shfl_sync(0xffffffffu, w, x);
-                if (s_part[x].have == 0) continue;
-                const float *part = part_of(x) + row * Plan::kPad + kC * lane;
+            for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            unsigned todo = members;
+            while (todo != 0) {
+                constexpr int kAtOnce = 4;
+                float wx[kAtOnce], from[kAtOnce][kC];
 #pragma unroll
-                for (int y = 0; y < kC; ++y) acc[y] += wx * part[y];
+                for (int n = 0; n < kAtOnce; ++n) {
+                    const int x = todo != 0 ? __ffs(todo) - 1 : 0;
+                    wx[n] = __shfl_sync(0xffffffffu, w, x);
+                    const float *part = x % 2 == 0 ? first_parts + x / 2 * Plan::kPartFloats : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
+#pragma unroll
+                    for (int y = 0; y < kC; ++y) from[n][y] = todo != 0 ? part[row * Plan::kPad + kC * lane + y] : 0.0f;
+                    if (todo == 0) wx[n] = 0.0f;
+                    todo &= todo - 1;
+                }
+#pragma unroll
+                for (int n = 0; n < kAtOnce; ++n)
+#pragma unroll
+                    for (int y = 0; y < kC; ++y) acc[y] += wx[n] * from[n][y];
             }
-            if (have == of.units) {
+            if (whole) {
                 T *out = static_cast<T *>(p.out) + of.seq * p.out_ld + (static_cast<long long>(of.head) * p.group + of.tile * Plan::kRows + row) * D + kC * lane;
                 const float inv = 1.0f / sum;
 #pragma unroll
                 for (int y = 0; y < kC; y += 2) *reinterpret_cast<uint32_t *>(out + y) = pack16<T>(acc[y] * inv, acc[y + 1] * inv);
-            } else {  // a CTA has at most one segment that began before it, and one that goes on behind it
-                const int slot = 2 * blockIdx.x + (of.start < c0 ? 0 : 1);
-                float *to = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
+            } else {
+                const int at = (2 * blockIdx.x + slot) * 16 + row;
+                float *to = p.partial + static_cast<size_t>(at) * D + kC * lane;
 #pragma unroll
                 for (int y = 0; y < kC; ++y) to[y] = acc[y];
-                if (lane == 0)
-                    *reinterpret_cast<float2 *>(p.partial + static_cast<size_t>(gridDim.x) * 2 * 16 * D + 2 * (slot * 16 + row)) = make_float2(top, sum);
+                if (lane == 0) *reinterpret_cast<float2 *>(p.partial + static_cast<size_t>(gridDim.x) * 2 * 16 * D + 2 * at) = make_float2(top, sum);
             }
         }
-        i = end;
+        nth += rows;
     }
+    if (threadIdx.x == 0) decode_crossings(p.partial, D, gridDim.x)[blockIdx.x] = crossing;
 }
 
 // Joins what several CTAs have of one segment.  Block (x, row): the segment that crosses from CTA x to the next, if x is the first
@@ -483,22 +515,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const Dec
     __shared__ float s_acc[kDecodeWarps][D];
     __shared__ float2 s_ml[kDecodeWarps];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.y, x0 = blockIdx.x;
-    // (the lengths are older than the kernel in front, which has waited for them)
-    const DecodeShare share = decode_share(p.cache, p.cache.kv_heads * p.q_tiles, ctas);
-    const long long c0 = share.begin(x0), c1 = share.begin(x0 + 1);
-    bool work = c0 < c1 && c1 < share.all;
-    DecodeAt at = {};
-    int r = 0;
-    if (work) {
-        at = decode_at(p.cache, p.q_tiles, c1);
-        r = at.tile * kRows + row;
-        work = at.unit > 0 && at.start >= c0 && r < p.group;
-    }
-    // (block 0 waits in any case: this kernel must not end before the one in front)
-    if (!work && (x0 > 0 || row > 0)) return;
     grid_dep_wait();
-    if (!work) return;
-    const int n = share.owner(at.start + at.units - 1) - x0 + 1;  // CTAs that have a part
+    const DecodeCrossing at = decode_crossings(p.partial, D, ctas)[x0];
+    const int r = at.tile * kRows + row, n = at.ctas;
+    if (n == 0 || r >= p.group) return;
     const float *ml = p.partial + static_cast<size_t>(ctas) * 2 * 16 * D;
     const auto slot_of = [&](int x) { return 2 * (x0 + x) + (x == 0 ? 1 : 0); };  // the segment begins in the first
     // the warp's own parts, eight at a time, with a maximum of its own: the loads wait for nothing but this kernel's start
