@@ -189,6 +189,15 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void load_floats(const float *p, float (&x)[4]) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+}
+__device__ __forceinline__ void load_floats(const float *p, float (&x)[2]) {
+    const float2 f = *reinterpret_cast<const float2 *>(p);
+    x[0] = f.x, x[1] = f.y;
+}
+
 // What a warp has of one segment when it could not write it out.
 struct DecodePart {
     long long start;
@@ -230,6 +239,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
 
         DecodeAt at = decode_at(p.cache, lens, p.q_tiles, u0), load = at;
         int left = static_cast<int>(u1 - u0);  // units not yet asked for
+        bool fresh_load = true;                // the next of them is the first of its segment
         const int32_t *table = p.cache.page_table + load.seq * p.cache.table_stride;
         int page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
         // The queries of a segment come with its first unit here, into one of two places in turn: at most two segments' are
@@ -248,41 +258,26 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 cp_async16_or_zero(dst + row * Plan::kRowBytes + ((piece ^ (row & 7)) << 4), have ? q + row * D : q, have);
             }
         };
-        issue_q();
         // asks for the unit at `load`, and goes on to the next, whose page number is then under way
-        bool fresh_load = false;
         const auto issue = [&](int stage) {
             if (fresh_load) issue_q();
             const int pos = load.unit * kUnitKeys, keys = load.len - pos;
             const bool there = page >= 0 && page < p.cache.num_pages;
             if (!there) raise_status(DMM_STATUS_BAD_PAGE);
+            const long long base = there ? page * p.cache.page_stride + load.head * p.cache.head_stride +
+                                               (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride + my_offset
+                                         : 0;
+            const T *k = static_cast<const T *>(p.cache.k) + base, *v = static_cast<const T *>(p.cache.v) + base;
             const uint32_t dst = ring + stage * 2 * Plan::kUnitBytes + row0 * Plan::kRowBytes;
-            if (there && keys >= kUnitKeys) {
-                const long long base = page * p.cache.page_stride + load.head * p.cache.head_stride +
-                                       (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride + my_offset;
-                const T *k = static_cast<const T *>(p.cache.k) + base, *v = static_cast<const T *>(p.cache.v) + base;
+            const int rows = there ? keys - row0 : 0;  // what is behind the sequence's end becomes zeros
 #pragma unroll
-                for (int i = 0; i < kUnitKeys / kRowsAtOnce; ++i) {
-                    const uint32_t d = dst + i * kRowsAtOnce * Plan::kRowBytes + ((piece ^ ((row0 + i * kRowsAtOnce) & 7)) << 4);
-                    cp_async16(d, k);
-                    cp_async16(d + Plan::kUnitBytes, v);
-                    k += step;
-                    v += step;
-                }
-            } else {  // the sequence's last unit: what is behind its end becomes zeros
-                const long long base = there ? page * p.cache.page_stride + load.head * p.cache.head_stride +
-                                                   (pos & ((1 << p.cache.page_shift) - 1)) * p.cache.row_stride
-                                             : 0;
-                const T *k = static_cast<const T *>(p.cache.k) + base, *v = static_cast<const T *>(p.cache.v) + base;
-#pragma unroll 1
-                for (int i = 0; i < kUnitKeys / kRowsAtOnce; ++i) {
-                    const int row = row0 + i * kRowsAtOnce;
-                    const bool have = there && row < keys;
-                    const uint32_t d = dst + i * kRowsAtOnce * Plan::kRowBytes + ((piece ^ (row & 7)) << 4);
-                    const long long off = have ? i * step + my_offset : 0;
-                    cp_async16_or_zero(d, k + off, have);
-                    cp_async16_or_zero(d + Plan::kUnitBytes, v + off, have);
-                }
+            for (int i = 0; i < kUnitKeys / kRowsAtOnce; ++i) {
+                const uint32_t d = dst + i * kRowsAtOnce * Plan::kRowBytes + ((piece ^ ((row0 + i * kRowsAtOnce) & 7)) << 4);
+                const bool have = i * kRowsAtOnce < rows;
+                cp_async16_or_zero(d, have ? k : static_cast<const T *>(p.cache.k), have);
+                cp_async16_or_zero(d + Plan::kUnitBytes, have ? v : static_cast<const T *>(p.cache.v), have);
+                k += step;
+                v += step;
             }
             if (--left > 0) {
                 fresh_load = decode_next(p.cache, p.q_tiles, load);
@@ -290,22 +285,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
             }
         };
-#pragma unroll
-        for (int s = 0; s < Plan::kStages - 1; ++s) {
-            if (left > 0) issue(s);
-            cp_async_commit();
-        }
-
         float o[kN][D / 16][4], m[kN][2], l[kN][2];
         uint32_t qf[kN][D / 16][2];
         int stage = 0, have = 0;
         bool fresh = true;
         const int a_row = ((lane / 8) % 2) * 8 + lane % 8, a_half = lane / 16;   // of K: (keys, 16-byte pieces) of the four tiles of a fragment
         const int v_row = (lane / 16) * 8 + lane % 8, v_half = (lane / 8) % 2;   // of V, which is read transposed
-        for (int n = static_cast<int>(u1 - u0); n > 0; --n) {
-            cp_async_wait<Plan::kStages - 2>();
-            __syncwarp();  // all lanes' pieces of this unit are there, and all have read the unit before
-            if (fresh) {
+        const int total = static_cast<int>(u1 - u0);
+        int fill = 0;
+        // (One copy of each step in the code, the first loads' too: a warp has few units, and instructions come from afar the
+        // first time.)
+        for (int n = 1 - Plan::kStages; n < total; ++n) {
+            if (n >= 0) {
+                cp_async_wait<Plan::kStages - 2>();
+                __syncwarp();  // all lanes' pieces of this unit are there, and all have read the unit before
+            }
+            if (n >= 0 && fresh) {
                 const uint32_t q = q_place + q_use * Plan::kQBytes;
                 q_use ^= 1;
 #pragma unroll
@@ -328,8 +323,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 have = 0;
                 __syncwarp();  // (the next queries but one come to this place)
             }
-            if (left > 0) issue(stage == 0 ? Plan::kStages - 1 : stage - 1);
+            if (left > 0) issue(fill);
             cp_async_commit();
+            if (++fill == Plan::kStages) fill = 0;
+            if (n < 0) continue;
 
             const uint32_t kb = ring + stage * 2 * Plan::kUnitBytes, vb = kb + Plan::kUnitBytes;
             float s[kN][2][4] = {};  // two chains of products, added at the end
@@ -396,8 +393,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             if (++stage == Plan::kStages) stage = 0;
             ++have;
 
-            if (at.unit + 1 == at.units || n == 1) {  // the end of the segment or of this warp's share
-                float *part = n > 1 ? first_parts + warp * Plan::kPartFloats : reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
+            if (at.unit + 1 == at.units || n + 1 == total) {  // the end of the segment or of this warp's share
+                float *part = n + 1 < total ? first_parts + warp * Plan::kPartFloats : reinterpret_cast<float *>(smem_raw + warp * Plan::kWarpBytes);
                 __syncwarp();  // (the last part lies where all lanes have read the last unit)
 #pragma unroll
                 for (int t = 0; t < kN; ++t) {
@@ -431,7 +428,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                         }
                     }
                 }
-                if (have != at.units && lane == 0) s_part[2 * warp + (n > 1 ? 0 : 1)] = {at.start, at.seq, at.head, at.tile, at.units, have};
+                if (have != at.units && lane == 0) s_part[2 * warp + (n + 1 < total ? 0 : 1)] = {at.start, at.seq, at.head, at.tile, at.units, have};
                 fresh = true;
             }
             decode_next(p.cache, p.q_tiles, at);
@@ -470,24 +467,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             float sum = w * ml.y, acc[kC] = {};
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            unsigned todo = members;
-            while (todo != 0) {
-                constexpr int kAtOnce = 4;
-                float wx[kAtOnce], from[kAtOnce][kC];
+#pragma unroll 1
+            for (unsigned todo = members; todo != 0; todo &= todo - 1) {
+                const int x = __ffs(todo) - 1;
+                const float wx = __shfl_sync(0xffffffffu, w, x);
+                float from[kC];
+                load_floats((x % 2 == 0 ? static_cast<const float *>(first_parts) + x / 2 * Plan::kPartFloats
+                                        : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes)) + row * Plan::kPad + kC * lane, from);
 #pragma unroll
-                for (int n = 0; n < kAtOnce; ++n) {
-                    const int x = todo != 0 ? __ffs(todo) - 1 : 0;
-                    wx[n] = __shfl_sync(0xffffffffu, w, x);
-                    const float *part = x % 2 == 0 ? first_parts + x / 2 * Plan::kPartFloats : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes);
-#pragma unroll
-                    for (int y = 0; y < kC; ++y) from[n][y] = todo != 0 ? part[row * Plan::kPad + kC * lane + y] : 0.0f;
-                    if (todo == 0) wx[n] = 0.0f;
-                    todo &= todo - 1;
-                }
-#pragma unroll
-                for (int n = 0; n < kAtOnce; ++n)
-#pragma unroll
-                    for (int y = 0; y < kC; ++y) acc[y] += wx[n] * from[n][y];
+                for (int y = 0; y < kC; ++y) acc[y] += wx * from[y];
             }
             if (whole) {
                 T *out = static_cast<T *>(p.out) + of.seq * p.out_ld + (static_cast<long long>(of.head) * p.group + of.tile * Plan::kRows + row) * D + kC * lane;
@@ -536,13 +524,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const Dec
             if (xi < n) {
                 v[i] = *reinterpret_cast<const float2 *>(ml + 2 * (slot * 16 + row));
                 const float *src = p.partial + (static_cast<size_t>(slot) * 16 + row) * D + kC * lane;
-                if constexpr (kC == 4) {
-                    const float4 f = *reinterpret_cast<const float4 *>(src);
-                    from[i][0] = f.x, from[i][1] = f.y, from[i][2] = f.z, from[i][3] = f.w;
-                } else {
-                    const float2 f = *reinterpret_cast<const float2 *>(src);
-                    from[i][0] = f.x, from[i][1] = f.y;
-                }
+                load_floats(src, from[i]);
             }
         }
         float to = top;
