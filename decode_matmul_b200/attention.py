@@ -37,9 +37,8 @@ def _no(msg: str):
 # A call on few tokens takes a few microseconds on the GPU: the checks ask every tensor once and make no text before it is needed.
 def _check_cache(k, v, table, lens):
     """Checks a cache and returns (its description for the library, dtype, device index, kv_heads, head_dim, sequences)."""
-    for t, name in ((k, "k_pages"), (v, "v_pages"), (table, "page_table"), (lens, "seq_lens")):
-        if not isinstance(t, torch.Tensor):
-            _no(f"{name} must be a tensor")
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(table, torch.Tensor) and isinstance(lens, torch.Tensor)):
+        _no("k_pages, v_pages, page_table and seq_lens must be tensors")
     dtype, index, shape, stride = k.dtype, k.get_device(), k.shape, k.stride()
     kind = _TYPE_16.get(dtype)
     if kind is None:
@@ -132,16 +131,16 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
             _no("freqs must be contiguous float64 [head_dim / 2]")
         if freqs.get_device() != index:
             _no("freqs must be on the device of k_pages")
+    if output is None:
+        output = k_pages.new_empty((tokens, heads, head_dim))
+        out_ld = heads * head_dim
+    else:
+        rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
+        if rows != tokens or out_heads != heads:
+            _no("output must be [tokens, heads, head_dim]")
+    if tokens == 0:
+        return output
     with _on_device_of(k_pages):
-        if output is None:
-            output = torch.empty((tokens, heads, head_dim), dtype=dtype, device=k_pages.device)
-            out_ld = heads * head_dim
-        else:
-            rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
-            if rows != tokens or out_heads != heads:
-                _no("output must be [tokens, heads, head_dim]")
-        if tokens == 0:
-            return output
         rc = _lib.lib().dmm_append_kv(qkv.data_ptr(), kind, qkv.stride(0) if tokens > 1 else width, tokens, heads,
                                       None if freqs is None else freqs.data_ptr(), 1 if interleaved else 0, output.data_ptr(), out_ld,
                                       ctypes.byref(cache), None if cu_seqlens is None else cu_seqlens.data_ptr(),
@@ -166,35 +165,36 @@ def _attend(name, q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, scale, 
         _check_cu(cu_seqlens, index, seqs)
     elif tokens != seqs:
         _no("q must have one row per sequence")
+    if output is None:
+        output = torch.empty_like(q) if q.is_contiguous() else q.new_empty((tokens, heads, head_dim))
+        out_ld = heads * head_dim
+    else:
+        rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
+        if rows != tokens or out_heads != heads:
+            _no("output must have the shape of q")
+        if tokens > 0 and output.data_ptr() == q.data_ptr():
+            _no("output must not be q")
+    if tokens == 0:
+        return output
+    if scale is None:
+        scale = head_dim ** -0.5
+    flags, stream = _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index)
     L = _lib.lib()
     with _on_device_of(k_pages):
-        if output is None:
-            output = torch.empty((tokens, heads, head_dim), dtype=dtype, device=k_pages.device)
-            out_ld = heads * head_dim
-        else:
-            rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
-            if rows != tokens or out_heads != heads:
-                _no("output must have the shape of q")
-            if tokens > 0 and output.data_ptr() == q.data_ptr():
-                _no("output must not be q")
-        if tokens == 0:
-            return output
-        need = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
         if workspace is None:
-            # scratch of this call's own: from the caching allocator, which knows about streams and captured graphs
-            if need:
-                workspace = torch.empty((need,), dtype=torch.uint8, device=k_pages.device)
+            # scratch of this call's own, of 16-bit values: the caching allocator knows about streams and captured graphs
+            ws_bytes = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
+            workspace = q.new_empty(((ws_bytes + 1) // 2,))
         elif not isinstance(workspace, torch.Tensor) or workspace.get_device() != index or not workspace.is_contiguous():
             _no(f"workspace must be a contiguous tensor on device {index}")
-        ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        scale = head_dim ** -0.5 if scale is None else float(scale)
-        flags, stream = _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index)
+        else:
+            ws_bytes = workspace.numel() * workspace.element_size()
         if cu_seqlens is None:
-            rc = L.dmm_paged_attention(q.data_ptr(), q_ld, heads, scale, output.data_ptr(), out_ld, ctypes.byref(cache), ws, ws_bytes,
-                                       flags, stream)
+            rc = L.dmm_paged_attention(q.data_ptr(), q_ld, heads, scale, output.data_ptr(), out_ld, ctypes.byref(cache),
+                                       workspace.data_ptr(), ws_bytes, flags, stream)
         else:
             rc = L.dmm_prompt_attention(q.data_ptr(), q_ld, tokens, heads, scale, output.data_ptr(), out_ld, ctypes.byref(cache),
-                                        cu_seqlens.data_ptr(), ws, ws_bytes, flags, stream)
+                                        cu_seqlens.data_ptr(), workspace.data_ptr(), ws_bytes, flags, stream)
     if rc:
         _lib.check(rc, name)
     return output
