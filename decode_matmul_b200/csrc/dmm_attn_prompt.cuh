@@ -48,7 +48,7 @@ struct PromptPlan {
     static constexpr uint32_t kRing = 2 * kTileBytes;
     static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
     static constexpr int kBarQ = 0, kBarFull = 2, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarP = kBarS + 2,
-                         kBarO = kBarP + 2, kBarGuard = kBarO + 2, kBarLook = kBarGuard + 1, kNumBars = kBarLook + kMostGuarded;
+                         kBarO = kBarP + 2, kBarGuard = kBarO + 2, kBarLook = kBarGuard + kMostGuarded, kNumBars = kBarLook + kMostGuarded;
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 64 + 1024;  // (the last: alignment)
     static constexpr uint32_t kS = 0, kO = 256;       // tensor memory columns: S of tile i at 128 i, O at 256 + D i
 };
@@ -82,20 +82,54 @@ __device__ __forceinline__ void mma_ts_f16_words(uint32_t d, uint32_t a, uint32_
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
-    uint32_t u[32];
+// 32 columns of a thread's row, not waited for
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *u) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
           "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
           "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
           "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
         : "r"(taddr)
         : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
+}
+// wait::ld that names 32 of the loaded registers, so that no use of them can be moved above it
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t *u) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]),
+                   "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]),
+                   "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]),
+                   "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two fp32 operations at once
+__device__ __forceinline__ uint64_t pair32(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair32(uint64_t r) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 // What a CTA works on.
@@ -168,7 +202,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             s_failed = 0;
             s_poison = 0;
             for (int i = 0; i < Plan::kNumBars; ++i)
-                mbar_init(bar(i), i >= Plan::kBarP && i < Plan::kBarP + 2 ? 4 : i == Plan::kBarGuard ? 2 : 1);
+                mbar_init(bar(i), i >= Plan::kBarP && i < Plan::kBarP + 2 ? 4 : i >= Plan::kBarGuard && i < Plan::kBarLook ? 2 : 1);
             fence_mbar_init();
         }
         __syncwarp();
@@ -289,7 +323,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (j < guarded)
                     mbar_wait(bar(Plan::kBarFull + (2 * j + 1) % Plan::kStages), phase(2 * j + 1), &s_failed);
                 else
-                    mbar_wait(bar(Plan::kBarGuard), static_cast<uint32_t>(j - guarded) & 1u, &s_failed);
+                    mbar_wait(bar(Plan::kBarGuard + j - guarded), 0, &s_failed);
                 const uint32_t v = lo(ring(2 * j + 1), Plan::kHalfBytes);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -353,7 +387,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Plan::kBarGuard));
+            if (lane == 0) mbar_arrive(bar(Plan::kBarGuard + j - guarded));
         }
     } else {
         // =============================== softmax ===============================
@@ -371,28 +405,37 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int j = 0; j < tiles[i]; ++j) {
             mbar_wait(bar(Plan::kBarS + i), static_cast<uint32_t>(j) & 1u, &s_failed);
             tc_fence_after();
-            const int rel = sees - j * kPromptKeys;
-            float top = -INFINITY;
+            uint32_t u[128];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, u + 32 * q);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_wait_ld32(u + 32 * q);
+            float s[128];
+#pragma unroll
+            for (int x = 0; x < 128; ++x) s[x] = __uint_as_float(u[x]);
+            if (turn != 1.0f)
+#pragma unroll
+                for (int x = 0; x < 128; ++x) s[x] *= turn;
+            if (j >= free) {
+                const int rel = sees - j * kPromptKeys;
+#pragma unroll
+                for (int x = 0; x < 128; ++x) s[x] = x < rel ? s[x] : -INFINITY;
+            }
+            float tops[4];  // (chains of their own)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float s[32];
-                tmem_ld32(s_at + 32 * q, s);
-                if (turn != 1.0f)
+                tops[q] = fmaxf(s[q], s[q + 4]);
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) s[x] *= turn;
-                if (j >= free)
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) s[x] = 32 * q + x < rel ? s[x] : -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 32; ++x) top = fmaxf(top, s[x]);
+                for (int x = 8; x < 128; x += 8) tops[q] = max3(tops[q], s[x + q], s[x + q + 4]);
             }
+            const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
             const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
             if (__any_sync(0xffffffffu, rise)) {
                 const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
                 m = to;
                 l *= f;
                 if (j > 0) {
-#pragma unroll
+#pragma unroll 1
                     for (int q = 0; q < D / 16; ++q) {
                         uint32_t o[16];
                         tmem_ld16(o_at + 16 * q, o);
@@ -403,26 +446,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                 }
             }
-            const float mc = m == -INFINITY ? 0.0f : m * c;
+            const float mc = m == -INFINITY ? 0.0f : -m * c;
+            const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
+            uint64_t sums[4] = {};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float s[32];
-                tmem_ld32(s_at + 32 * q, s);
-                if (turn != 1.0f)
+            for (int q = 0; q < 8; ++q) {
+                uint32_t w[8];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) s[x] *= turn;
-                if (j >= free)
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) s[x] = 32 * q + x < rel ? s[x] : -INFINITY;
-                uint32_t w[16];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const float a = exp2_fast(fmaf(s[2 * x], c, -mc)), b = exp2_fast(fmaf(s[2 * x + 1], c, -mc));
-                    l += a + b;
+                for (int x = 0; x < 8; ++x) {
+                    const float2 y = unpair32(fma2(pair32(s[16 * q + 2 * x], s[16 * q + 2 * x + 1]), c2, mc2));
+                    const float a = exp2_fast(y.x), b = exp2_fast(y.y);
+                    sums[x % 4] = add2(sums[x % 4], pair32(a, b));
                     w[x] = pack16<T>(a, b);
                 }
-                tmem_st16(s_at + 16 * q, w);
+                tmem_st8(s_at + 8 * q, w);
             }
+            const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+            l += sum.x + sum.y;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -436,13 +476,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + r % p.group) * D;
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
+            uint32_t u[32];
             float o[32];
             if (tiles[i] > 0) {
-                tmem_ld32(o_at + 32 * q, o);
-            } else {
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = 0.0f;
+                tmem_ld32(o_at + 32 * q, u);
+                tmem_wait_ld32(u);
             }
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = tiles[i] > 0 ? __uint_as_float(u[x]) : 0.0f;
             if (s_poison && mine) {
                 for (int pos = guarded * kPromptKeys; pos < sees; ++pos) {
                     const long long row = cache_row(p.cache, it.seq, pos, it.head);
