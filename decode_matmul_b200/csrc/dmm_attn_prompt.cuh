@@ -47,8 +47,19 @@ struct PromptPlan {
     static constexpr uint32_t kQ = 0;
     static constexpr uint32_t kRing = 2 * kTileBytes;
     static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
-    static constexpr int kBarQ = 0, kBarFull = 2, kBarEmpty = kBarFull + kStages, kBarS = kBarEmpty + kStages, kBarP = kBarS + 2,
-                         kBarO = kBarP + 2, kBarGuard = kBarO + 2, kBarLook = kBarGuard + kMostGuarded, kNumBars = kBarLook + kMostGuarded;
+    // Barriers, in the order of their use for an item.  What not every item uses twice in a row has a phase of its own, which its users
+    // count; the guard's come in two sets that the items use in turn.
+    static constexpr int kBarItem = 0, kBarItemFree = 2, kBarNext = 4, kBarQ = 5, kBarQFree = 7, kBarFull = 9, kBarEmpty = kBarFull + kStages,
+                         kBarS = kBarEmpty + kStages, kBarP = kBarS + 2, kBarO = kBarP + 2, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
+                         kBarGuard = kBarLook + 2 * kMostGuarded, kNumBars = kBarGuard + 2 * kMostGuarded;
+    __device__ static constexpr int phase_bit(int item, int tile) { return (item & 1) * kMostGuarded + tile; }
+    __device__ static constexpr int look(int item, int tile) { return kBarLook + phase_bit(item, tile); }
+    __device__ static constexpr int guard(int item, int tile) { return kBarGuard + phase_bit(item, tile); }
+    __device__ static constexpr uint32_t arrivals(int bar) {
+        if (bar >= kBarItemFree && bar < kBarNext) return 11;  // every warp but the one that finds the items
+        if ((bar >= kBarP && bar < kBarO) || (bar >= kBarOFree && bar < kBarLook)) return 4;
+        return bar >= kBarGuard ? 2 : 1;
+    }
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 64 + 1024;  // (the last: alignment)
     static constexpr uint32_t kS = 0, kO = 256;       // tensor memory columns: S of tile i at 128 i, O at 256 + D i
 };
@@ -181,334 +192,457 @@ struct F16Kind<__nv_bfloat16> {
     static constexpr uint32_t kType = (1u << 7) | (1u << 10), kExponent = 0x7F80u;
 };
 
+// The next block of the grid that has not begun, taken over (cluster launch control): asked for, and the answer, -1 when there is none.
+__device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
+    fence_async_smem();  // (the answer before has been read)
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int next_block(uint32_t answer) {
+    int x;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b128 r;\nld.shared.b128 r, [%1];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\nmov.b32 %0, -1;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n}\n"
+        : "=r"(x)
+        : "r"(answer)
+        : "memory");
+    return x;
+}
+
+// What follows from an item: the key tiles of each of its two tiles, how many keys their last rows see, and the first key tile in which
+// a row ends (or the sequence).  Row t of the new tokens sees keys below len - n + t + 1.
+struct PromptExtent {
+    int tiles[2], most[2], all, guarded;
+    __device__ __forceinline__ PromptExtent(const PromptItem &it, int tile_tokens) {
+        const int shift = it.len - it.n + 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t0 = it.token0 + i * tile_tokens, t1 = min(t0 + tile_tokens, it.n);
+            most[i] = t1 > t0 ? max(0, shift + t1 - 1) : 0;
+            tiles[i] = (most[i] + kPromptKeys - 1) / kPromptKeys;
+        }
+        all = max(tiles[0], tiles[1]);
+        guarded = max(0, shift + it.token0) / kPromptKeys;
+    }
+};
+
+// A CTA goes from item to item: the loads of the next begin while the tensor cores are still at work on the present one.  The load
+// warp finds the items and hands them on in two places in turn.
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap, const PromptParams p) {
     using Plan = PromptPlan<D>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ PromptItem s_item;
+    __shared__ PromptItem s_item[2];
+    __shared__ __align__(16) uint32_t s_answer[4];
     __shared__ uint32_t s_tmem;
-    __shared__ volatile int s_failed, s_poison;
+    __shared__ volatile int s_failed, s_poison[2];
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tt = p.tile_tokens;
     const auto bar = [&](int i) { return smem + Plan::kBars + 8u * static_cast<uint32_t>(i); };
     grid_dep_wait();
-    if (warp == 0) {
-        const PromptItem it = prompt_item(p, static_cast<int>(blockIdx.x));
-        if (lane == 0) s_item = it;
-    } else if (warp == 8) {
+    if (warp == 8) {
         if (lane == 0) {
             s_failed = 0;
-            s_poison = 0;
-            for (int i = 0; i < Plan::kNumBars; ++i)
-                mbar_init(bar(i), i >= Plan::kBarP && i < Plan::kBarP + 2 ? 4 : i >= Plan::kBarGuard && i < Plan::kBarLook ? 2 : 1);
+            for (int i = 0; i < Plan::kNumBars; ++i) mbar_init(bar(i), Plan::arrivals(i));
             fence_mbar_init();
         }
         __syncwarp();
+        tmem_alloc(smem_u32(&s_tmem), 512);
     }
-    __syncthreads();
-    const PromptItem it = s_item;
-    if (it.seq < 0) return;
-    if (warp == 8) tmem_alloc(smem_u32(&s_tmem), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.
+    const auto item_of = [&](int k) {
+        mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed);
+        PromptItem it = s_item[k & 1];
+        if (s_failed) it.seq = -1;
+        return it;
+    };
+    const auto item_done = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Plan::kBarItemFree + (k & 1)));
+    };
 
-    // Row i of the new tokens sees keys below len - n + i + 1.  first, last: of the tokens of a tile that exist.
-    const int shift = it.len - it.n + 1, tt = p.tile_tokens;
-    const auto limit = [&](int token) { return shift + token; };
-    int tiles[2], most[2];  // key tiles, and keys that the last row sees
+    // Registers: 384 threads are launched with 168 each; the softmax holds a row of 128 scores and wants more, the others need
+    // less (256 * 208 + 128 * 80 = 63488 of 64512).
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 9) {
+            // =============================== items and loads ===============================
+            const int shift_pg = p.cache.page_shift, page = 1 << shift_pg, box = min(page, kPromptKeys);
+            int index = static_cast<int>(blockIdx.x), stage = 0;
+            uint32_t parity = 1, q_free = 0;  // q_free: bits, phases
+            bool q_used[2] = {false, false};
+            for (int k = 0;; ++k) {
+                PromptItem it = {-1, 0, 0, 0, 0, 0};
+                if (index >= 0) it = prompt_item(p, index);
+                if (k >= 2) mbar_wait(bar(Plan::kBarItemFree + (k & 1)), static_cast<uint32_t>((k >> 1) - 1) & 1u, &s_failed);
+                if (s_failed) it.seq = -1;
+                if (lane == 0) {
+                    s_item[k & 1] = it;
+                    s_poison[k & 1] = 0;
+                    mbar_arrive(bar(Plan::kBarItem + (k & 1)));
+                }
+                if (it.seq < 0) {
+                    // blocks behind the last item need not begin at all
+                    for (; index >= 0 && !s_failed; ++k) {
+                        if (lane == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
+                        __syncwarp();
+                        mbar_wait(bar(Plan::kBarNext), static_cast<uint32_t>(k) & 1u, &s_failed);
+                        index = next_block(smem_u32(s_answer));
+                        __syncwarp();
+                    }
+                    break;
+                }
+                const PromptExtent ext(it, tt);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t0 = it.token0 + i * tt, t1 = min(t0 + tt, it.n);
-        most[i] = t1 > t0 ? max(0, limit(t1 - 1)) : 0;
-        tiles[i] = (most[i] + kPromptKeys - 1) / kPromptKeys;
-    }
-    const int all = max(tiles[0], tiles[1]);
-    // the first key tile in which a row ends, or the sequence; the values of these tiles arrive at barriers of their own, for the guard
-    const int guarded = max(0, limit(it.token0)) / kPromptKeys;
-
-    if (warp == 9) {
-        // =============================== loads ===============================
-        if (all > 0) {
-            if (lane == 0) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (tiles[i] > 0) {
+                for (int i = 0; i < 2; ++i) {
+                    if (ext.tiles[i] == 0) continue;
+                    if (q_used[i]) {  // the products of the item before that used this place are done with it
+                        mbar_wait(bar(Plan::kBarQFree + i), (q_free >> i) & 1u, &s_failed);
+                        q_free ^= 1u << i;
+                    }
+                    q_used[i] = true;
+                    if (lane == 0) {
                         mbar_arrive_expect_tx(bar(Plan::kBarQ + i), static_cast<uint32_t>(Plan::kHalves * p.group * tt) * 128u);
 #pragma unroll
                         for (int hh = 0; hh < Plan::kHalves; ++hh)
                             tma_load_3d(smem + Plan::kQ + i * Plan::kTileBytes + hh * Plan::kHalfBytes, &qmap, 64 * hh, it.head * p.group,
                                         it.begin + it.token0 + i * tt, bar(Plan::kBarQ + i));
                     }
-            }
-            const int shift_pg = p.cache.page_shift, page = 1 << shift_pg, box = min(page, kPromptKeys);
-            const int32_t *table = p.cache.page_table + it.seq * p.cache.table_stride;
-            int stage = 0;
-            uint32_t parity = 1;
-            for (int j = 0; j < all; ++j) {
-                const int pos = j * kPromptKeys + lane * box;
-                const bool mine = lane * box < kPromptKeys && pos < it.len;
-                int pg = 0;
-                if (mine) {
-                    pg = table[pos >> shift_pg];
-                    if (pg < 0 || pg >= p.cache.num_pages) {
-                        raise_status(DMM_STATUS_BAD_PAGE);
-                        pg = -1;  // outside the tensor map: reads as zeros
-                    }
                 }
-                const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine)) * box) * 128u * Plan::kHalves;
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    mbar_wait(bar(Plan::kBarEmpty + stage), parity, &s_failed);
-                    const uint32_t full = bar(kv == 1 && j >= guarded ? Plan::kBarLook + j - guarded : Plan::kBarFull + stage);
-                    if (lane == 0) mbar_arrive_expect_tx(full, bytes);
-                    __syncwarp();
+                const int32_t *table = p.cache.page_table + it.seq * p.cache.table_stride;
+                if (lane == 0 && ext.all == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
+                for (int j = 0; j < ext.all; ++j) {
+                    if (lane == 0 && j + 1 == ext.all) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
+                    const int pos = j * kPromptKeys + lane * box;
+                    const bool mine = lane * box < kPromptKeys && pos < it.len;
+                    int pg = 0;
                     if (mine) {
-                        const uint32_t dst = smem + Plan::kRing + stage * Plan::kTileBytes + static_cast<uint32_t>(lane * box) * 128u;
-#pragma unroll
-                        for (int hh = 0; hh < Plan::kHalves; ++hh)
-                            tma_load_4d(dst + hh * Plan::kHalfBytes, kv == 0 ? &kmap : &vmap, 64 * hh, pos & (page - 1), it.head, pg, full);
-                    }
-                    if (++stage == Plan::kStages) {
-                        stage = 0;
-                        parity ^= 1u;
-                    }
-                }
-            }
-            if (s_failed) {  // a wait gave up: let the copies in flight land before the CTA goes
-                for (int j = all; j-- > 0 && j >= all - Plan::kStages;) {
-                    mbar_wait_limit(bar(Plan::kBarFull + 2 * j % Plan::kStages), static_cast<uint32_t>(2 * j / Plan::kStages) & 1u, kWaitLimitCycles);
-                    if (j >= guarded) mbar_wait_limit(bar(Plan::kBarLook + j - guarded), 0, kWaitLimitCycles);
-                    else mbar_wait_limit(bar(Plan::kBarFull + (2 * j + 1) % Plan::kStages), static_cast<uint32_t>((2 * j + 1) / Plan::kStages) & 1u, kWaitLimitCycles);
-                }
-            }
-        }
-    } else if (warp == 8) {
-        // =============================== MMA ===============================
-        const bool leader = elect_one();
-        // D fp32 (1 at bit 4), the operands' type, N >> 3 at bit 17, M >> 4 at bit 24; V is the operand whose rows run along N (bit 16)
-        constexpr uint32_t kIdS = (1u << 4) | F16Kind<T>::kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-        constexpr uint32_t kIdO = (1u << 4) | F16Kind<T>::kType | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
-        // 128-byte swizzle (2 at bit 61), 8-row groups 1024 bytes apart, version 1 at bit 46; the low word has the address and, for
-        // V, the distance from one 64 columns to the next
-        constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-        const auto lo = [&](uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); };
-        const auto ring = [&](int n) { return smem + Plan::kRing + static_cast<uint32_t>(n % Plan::kStages) * Plan::kTileBytes; };
-        const auto phase = [&](int n) { return static_cast<uint32_t>(n / Plan::kStages) & 1u; };
-        const auto scores = [&](int i, int j) {
-            const uint32_t a = lo(smem + Plan::kQ + i * Plan::kTileBytes, 16), b = lo(ring(2 * j), 16);
-            if (leader) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k / 4) * (Plan::kHalfBytes >> 4) + (k % 4) * 2;
-                    mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, kIdS, k > 0);
-                }
-                tc_commit(bar(Plan::kBarS + i));
-            }
-        };
-        if (all > 0) {
-            mbar_wait(bar(Plan::kBarFull), 0, &s_failed);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (tiles[i] > 0) {
-                    mbar_wait(bar(Plan::kBarQ + i), 0, &s_failed);
-                    tc_fence_after();
-                    scores(i, 0);
-                }
-            if (leader) tc_commit(bar(Plan::kBarEmpty));
-            for (int j = 0; j < all; ++j) {
-                if (j < guarded)
-                    mbar_wait(bar(Plan::kBarFull + (2 * j + 1) % Plan::kStages), phase(2 * j + 1), &s_failed);
-                else
-                    mbar_wait(bar(Plan::kBarGuard + j - guarded), 0, &s_failed);
-                const uint32_t v = lo(ring(2 * j + 1), Plan::kHalfBytes);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (j < tiles[i]) {
-                        mbar_wait(bar(Plan::kBarP + i), static_cast<uint32_t>(j) & 1u, &s_failed);
-                        tc_fence_after();
-                        if (leader) {
-                            // (the last tile: only the 16 keys at a time that some row sees)
-                            const int steps = min(8, (most[i] - j * kPromptKeys + 15) / 16);
-                            for (int k = 0; k < steps; ++k)
-                                mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * k, v + k * (2048u >> 4), kHi, kIdO, j > 0 || k > 0);
-                            if (j + 1 == tiles[i]) tc_commit(bar(Plan::kBarO + i));
+                        pg = table[pos >> shift_pg];
+                        if (pg < 0 || pg >= p.cache.num_pages) {
+                            raise_status(DMM_STATUS_BAD_PAGE);
+                            pg = -1;  // outside the tensor map: reads as zeros
                         }
-                        __syncwarp();
                     }
-                    if (j + 1 < tiles[i]) {
-                        mbar_wait(bar(Plan::kBarFull + (2 * j + 2) % Plan::kStages), phase(2 * j + 2), &s_failed);
-                        tc_fence_after();
-                        scores(i, j + 1);
-                    }
-                }
-                if (leader) {
-                    tc_commit(bar(Plan::kBarEmpty + (2 * j + 1) % Plan::kStages));
-                    if (j + 1 < all) tc_commit(bar(Plan::kBarEmpty + (2 * j + 2) % Plan::kStages));
-                }
-            }
-        }
-    } else if (warp >= 10) {
-        // =============================== guard ===============================
-        const int t = threadIdx.x - 320;
-        constexpr uint32_t kMask = F16Kind<T>::kExponent * 0x10001u;
-        for (int j = guarded; j < all; ++j) {
-            const int n = 2 * j + 1, rows = min(kPromptKeys, it.len - j * kPromptKeys);
-            mbar_wait(bar(Plan::kBarLook + j - guarded), 0, &s_failed);
-            const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>(n % Plan::kStages) * Plan::kTileBytes;
-            const auto where = [&](int c) { return base + (c / 1024) * Plan::kHalfBytes + (c % 1024) * 16u; };  // piece c: row (c % 1024) / 8
-            const auto bad = [](uint32_t w) { return (w & 0xFFFFu & kMask) == (kMask & 0xFFFFu) || (w & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u); };
-            bool any = false;
-            for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
-                const int row = (c % 1024) / 8;
-                if (row < rows) {
-                    const uint4 w = lds128(where(c));
-                    any |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
-                } else if (row < ((rows + 15) & ~15)) {
-                    sts128(where(c), make_uint4(0, 0, 0, 0));
-                }
-            }
-            if (any) {
-                s_poison = 1;
-                for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
-                    if ((c % 1024) / 8 >= rows) continue;
-                    const uint4 w = lds128(where(c));
-                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                    const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine)) * box) * 128u * Plan::kHalves;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if ((x[i] & 0xFFFFu & kMask) == (kMask & 0xFFFFu)) x[i] &= 0xFFFF0000u;
-                        if ((x[i] & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u)) x[i] &= 0xFFFFu;
+                    for (int kv = 0; kv < 2; ++kv) {
+                        mbar_wait(bar(Plan::kBarEmpty + stage), parity, &s_failed);
+                        if (s_failed) break;
+                        // (values that the guard looks at first arrive at barriers of their own)
+                        const uint32_t full = bar(kv == 1 && j >= ext.guarded ? Plan::look(k, j - ext.guarded) : Plan::kBarFull + stage);
+                        if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+                        __syncwarp();
+                        if (mine) {
+                            const uint32_t dst = smem + Plan::kRing + stage * Plan::kTileBytes + static_cast<uint32_t>(lane * box) * 128u;
+#pragma unroll
+                            for (int hh = 0; hh < Plan::kHalves; ++hh)
+                                tma_load_4d(dst + hh * Plan::kHalfBytes, kv == 0 ? &kmap : &vmap, 64 * hh, pos & (page - 1), it.head, pg, full);
+                        }
+                        if (kv == 1 && j >= ext.guarded && lane == 0) mbar_arrive(bar(Plan::kBarFull + stage));  // (keeps its phases in step)
+                        if (++stage == Plan::kStages) {
+                            stage = 0;
+                            parity ^= 1u;
+                        }
                     }
-                    sts128(where(c), make_uint4(x[0], x[1], x[2], x[3]));
                 }
+                mbar_wait(bar(Plan::kBarNext), static_cast<uint32_t>(k) & 1u, &s_failed);
+                index = next_block(smem_u32(s_answer));
+                __syncwarp();
             }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Plan::kBarGuard + j - guarded));
+            if (s_failed) {  // a wait gave up: copies in flight land before the CTA goes (they take microseconds)
+                const long long t0 = clock64();
+                while (clock64() - t0 < 4000000) __nanosleep(1000);
+            }
+        } else if (warp == 8) {
+            // =============================== MMA ===============================
+            const bool leader = elect_one();
+            // D fp32 (1 at bit 4), the operands' type, N >> 3 at bit 17, M >> 4 at bit 24; V is the operand whose rows run along N (bit 16)
+            constexpr uint32_t kIdS = (1u << 4) | F16Kind<T>::kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t kIdO = (1u << 4) | F16Kind<T>::kType | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
+            // 128-byte swizzle (2 at bit 61), 8-row groups 1024 bytes apart, version 1 at bit 46; the low word has the address and, for
+            // V, the distance from one 64 columns to the next
+            constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+            const auto lo = [&](uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); };
+            // the ring's next tile: where it is, and the wait for it
+            int stage = 0;
+            uint32_t parity = 0;
+            const auto place = [&](int s) { return smem + Plan::kRing + static_cast<uint32_t>(s) * Plan::kTileBytes; };
+            const auto step = [&]() {
+                if (++stage == Plan::kStages) {
+                    stage = 0;
+                    parity ^= 1u;
+                }
+            };
+            const auto scores = [&](int i, int s) {
+                const uint32_t a = lo(smem + Plan::kQ + i * Plan::kTileBytes, 16), b = lo(place(s), 16);
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = (k / 4) * (Plan::kHalfBytes >> 4) + (k % 4) * 2;
+                        mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, kIdS, k > 0);
+                    }
+                    tc_commit(bar(Plan::kBarS + i));
+                }
+            };
+            uint32_t q_full = 0, p_full = 0, o_free = 0, guard = 0;  // bits: phases
+            bool o_used[2] = {false, false};
+            for (int k = 0;; ++k) {
+                const PromptItem it = item_of(k);
+                if (it.seq < 0) break;
+                const PromptExtent ext(it, tt);
+                if (ext.all > 0) {
+                    mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (ext.tiles[i] > 0) {
+                            mbar_wait(bar(Plan::kBarQ + i), (q_full >> i) & 1u, &s_failed);
+                            q_full ^= 1u << i;
+                            tc_fence_after();
+                            scores(i, stage);
+                            if (leader && ext.tiles[i] == 1) tc_commit(bar(Plan::kBarQFree + i));
+                        }
+                    if (leader) tc_commit(bar(Plan::kBarEmpty + stage));
+                    step();
+                }
+                for (int j = 0; j < ext.all; ++j) {
+                    mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
+                    if (j >= ext.guarded) {
+                        const int g = j - ext.guarded, at = Plan::phase_bit(k, g);
+                        mbar_wait(bar(Plan::guard(k, g)), (guard >> at) & 1u, &s_failed);
+                        guard ^= 1u << at;
+                    }
+                    const int v_stage = stage;
+                    const uint32_t v = lo(place(v_stage), Plan::kHalfBytes);
+                    step();
+                    bool k_there = false;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (j < ext.tiles[i]) {
+                            if (j == 0) {  // the epilogue before has read O
+                                if (o_used[i]) {
+                                    mbar_wait(bar(Plan::kBarOFree + i), (o_free >> i) & 1u, &s_failed);
+                                    o_free ^= 1u << i;
+                                }
+                                o_used[i] = true;
+                            }
+                            mbar_wait(bar(Plan::kBarP + i), (p_full >> i) & 1u, &s_failed);
+                            p_full ^= 1u << i;
+                            tc_fence_after();
+                            if (leader) {
+                                // (the last tile: only the 16 keys at a time that some row sees)
+                                const int steps = min(8, (ext.most[i] - j * kPromptKeys + 15) / 16);
+                                for (int n = 0; n < steps; ++n)
+                                    mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * n, v + n * (2048u >> 4), kHi, kIdO, j > 0 || n > 0);
+                                if (j + 1 == ext.tiles[i]) tc_commit(bar(Plan::kBarO + i));
+                            }
+                            __syncwarp();
+                        }
+                        if (j + 1 < ext.tiles[i]) {
+                            if (!k_there) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
+                            k_there = true;
+                            tc_fence_after();
+                            scores(i, stage);
+                            if (leader && j + 2 == ext.tiles[i]) tc_commit(bar(Plan::kBarQFree + i));
+                        }
+                    }
+                    if (leader) {
+                        tc_commit(bar(Plan::kBarEmpty + v_stage));
+                        if (k_there) tc_commit(bar(Plan::kBarEmpty + stage));
+                    }
+                    if (k_there) step();
+                }
+                item_done(k);
+            }
+        } else if (warp >= 10) {
+            // =============================== guard ===============================
+            const int t = threadIdx.x - 320;
+            constexpr uint32_t kMask = F16Kind<T>::kExponent * 0x10001u;
+            int tile0 = 0;        // tiles of the ring that items before had
+            uint32_t look = 0;    // bits: phases
+            for (int k = 0;; ++k) {
+                const PromptItem it = item_of(k);
+                if (it.seq < 0) break;
+                const PromptExtent ext(it, tt);
+                for (int j = ext.guarded; j < ext.all; ++j) {
+                    const int rows = min(kPromptKeys, it.len - j * kPromptKeys), g = j - ext.guarded, at = Plan::phase_bit(k, g);
+                    mbar_wait(bar(Plan::look(k, g)), (look >> at) & 1u, &s_failed);
+                    look ^= 1u << at;
+                    const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>((tile0 + 2 * j + 1) % Plan::kStages) * Plan::kTileBytes;
+                    const auto where = [&](int c) { return base + (c / 1024) * Plan::kHalfBytes + (c % 1024) * 16u; };  // piece c: row (c % 1024) / 8
+                    const auto bad = [](uint32_t w) { return (w & 0xFFFFu & kMask) == (kMask & 0xFFFFu) || (w & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u); };
+                    bool any = false;
+                    for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
+                        const int row = (c % 1024) / 8;
+                        if (row < rows) {
+                            const uint4 w = lds128(where(c));
+                            any |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+                        } else if (row < ((rows + 15) & ~15)) {
+                            sts128(where(c), make_uint4(0, 0, 0, 0));
+                        }
+                    }
+                    if (any) {
+                        s_poison[k & 1] = 1;
+                        for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
+                            if ((c % 1024) / 8 >= rows) continue;
+                            const uint4 w = lds128(where(c));
+                            uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if ((x[i] & 0xFFFFu & kMask) == (kMask & 0xFFFFu)) x[i] &= 0xFFFF0000u;
+                                if ((x[i] & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u)) x[i] &= 0xFFFFu;
+                            }
+                            sts128(where(c), make_uint4(x[0], x[1], x[2], x[3]));
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(Plan::guard(k, g)));
+                }
+                tile0 = (tile0 + 2 * ext.all) % Plan::kStages;
+                item_done(k);
+            }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // =============================== softmax ===============================
         const int i = warp / 4, r = threadIdx.x % 128, tok = r / p.group;
-        const int token = it.token0 + i * tt + tok;
-        const bool mine = tok < tt && token < it.n;
-        const int sees = mine ? max(0, limit(token)) : 0;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
         const uint32_t s_at = lanes + Plan::kS + 128 * i, o_at = lanes + Plan::kO + D * i;
         // c S <= 0 for c <= 0: such scales turn the sign of S, or make it 0
         const float turn = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
         const float c = turn == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
-        const int free = max(0, limit(it.token0 + i * tt)) / kPromptKeys;  // key tiles that every row of this tile sees whole
-        float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < tiles[i]; ++j) {
-            mbar_wait(bar(Plan::kBarS + i), static_cast<uint32_t>(j) & 1u, &s_failed);
-            tc_fence_after();
-            uint32_t u[128];
+        uint32_t s_full = 0, o_full = 0;  // phases
+        for (int k = 0;; ++k) {
+            const PromptItem it = item_of(k);
+            if (it.seq < 0) break;
+            const PromptExtent ext(it, tt);
+            const int tiles = i == 0 ? ext.tiles[0] : ext.tiles[1];
+            const int token = it.token0 + i * tt + tok, shift = it.len - it.n + 1;
+            const bool mine = tok < tt && token < it.n;
+            const int sees = mine ? max(0, shift + token) : 0;
+            const int free = max(0, shift + it.token0 + i * tt) / kPromptKeys;  // key tiles that every row of this tile sees whole
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < tiles; ++j) {
+                mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
+                s_full ^= 1u;
+                tc_fence_after();
+                uint32_t u[128];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, u + 32 * q);
+                for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, u + 32 * q);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_wait_ld32(u + 32 * q);
-            float s[128];
+                for (int q = 0; q < 4; ++q) tmem_wait_ld32(u + 32 * q);
+                float s[128];
 #pragma unroll
-            for (int x = 0; x < 128; ++x) s[x] = __uint_as_float(u[x]);
-            if (turn != 1.0f)
+                for (int x = 0; x < 128; ++x) s[x] = __uint_as_float(u[x]);
+                if (turn != 1.0f)
 #pragma unroll
-                for (int x = 0; x < 128; ++x) s[x] *= turn;
-            if (j >= free) {
-                const int rel = sees - j * kPromptKeys;
+                    for (int x = 0; x < 128; ++x) s[x] *= turn;
+                if (j >= free) {
+                    const int rel = sees - j * kPromptKeys;
 #pragma unroll
-                for (int x = 0; x < 128; ++x) s[x] = x < rel ? s[x] : -INFINITY;
-            }
-            float tops[4];  // (chains of their own)
+                    for (int x = 0; x < 128; ++x) s[x] = x < rel ? s[x] : -INFINITY;
+                }
+                float tops[4];  // (chains of their own)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                tops[q] = fmaxf(s[q], s[q + 4]);
+                for (int q = 0; q < 4; ++q) {
+                    tops[q] = fmaxf(s[q], s[q + 4]);
 #pragma unroll
-                for (int x = 8; x < 128; x += 8) tops[q] = max3(tops[q], s[x + q], s[x + q + 4]);
-            }
-            const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
-            const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
-            if (__any_sync(0xffffffffu, rise)) {
-                const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
-                m = to;
-                l *= f;
-                if (j > 0) {
+                    for (int x = 8; x < 128; x += 8) tops[q] = max3(tops[q], s[x + q], s[x + q + 4]);
+                }
+                const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
+                const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
+                    m = to;
+                    l *= f;
+                    if (j > 0) {
 #pragma unroll 1
-                    for (int q = 0; q < D / 16; ++q) {
-                        uint32_t o[16];
-                        tmem_ld16(o_at + 16 * q, o);
-                        tmem_wait_ld(o);
+                        for (int q = 0; q < D / 16; ++q) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + 16 * q, o);
+                            tmem_wait_ld(o);
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                        tmem_st16(o_at + 16 * q, o);
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            tmem_st16(o_at + 16 * q, o);
+                        }
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.0f : -m * c;
+                const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
+                uint64_t sums[4] = {};
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const float2 y = unpair32(fma2(pair32(s[16 * q + 2 * x], s[16 * q + 2 * x + 1]), c2, mc2));
+                        const float a = exp2_fast(y.x), b = exp2_fast(y.y);
+                        sums[x % 4] = add2(sums[x % 4], pair32(a, b));
+                        w[x] = pack16<T>(a, b);
+                    }
+                    tmem_st8(s_at + 8 * q, w);
+                }
+                const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+                l += sum.x + sum.y;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(Plan::kBarP + i));
+            }
+            if (tiles > 0) {
+                mbar_wait(bar(Plan::kBarO + i), o_full, &s_failed);
+                o_full ^= 1u;
+                tc_fence_after();
+            }
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + r % p.group) * D;
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t u[32];
+                float o[32];
+                if (tiles > 0) {
+                    tmem_ld32(o_at + 32 * q, u);
+                    tmem_wait_ld32(u);
+                }
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = tiles > 0 ? __uint_as_float(u[x]) : 0.0f;
+                if (s_poison[k & 1] && mine) {
+                    for (int pos = ext.guarded * kPromptKeys; pos < sees; ++pos) {
+                        const long long row = cache_row(p.cache, it.seq, pos, it.head);
+                        if (row < 0) continue;
+                        const T *v = static_cast<const T *>(p.cache.v) + row + 32 * q;
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            const float f = static_cast<float>(v[x]);
+                            if (!isfinite(f)) o[x] += f;
+                        }
+                    }
+                }
+                if (mine) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) y[z] = o[x + z] * inv;
+                        *reinterpret_cast<uint4 *>(out + 32 * q + x) =
+                            make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
                     }
                 }
             }
-            const float mc = m == -INFINITY ? 0.0f : -m * c;
-            const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
-            uint64_t sums[4] = {};
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                uint32_t w[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const float2 y = unpair32(fma2(pair32(s[16 * q + 2 * x], s[16 * q + 2 * x + 1]), c2, mc2));
-                    const float a = exp2_fast(y.x), b = exp2_fast(y.y);
-                    sums[x % 4] = add2(sums[x % 4], pair32(a, b));
-                    w[x] = pack16<T>(a, b);
-                }
-                tmem_st8(s_at + 8 * q, w);
-            }
-            const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-            l += sum.x + sum.y;
-            tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Plan::kBarP + i));
+            if (lane == 0 && tiles > 0) mbar_arrive(bar(Plan::kBarOFree + i));
+            item_done(k);
         }
-        if (tiles[i] > 0) {
-            mbar_wait(bar(Plan::kBarO + i), 0, &s_failed);
-            tc_fence_after();
-        }
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + r % p.group) * D;
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-            uint32_t u[32];
-            float o[32];
-            if (tiles[i] > 0) {
-                tmem_ld32(o_at + 32 * q, u);
-                tmem_wait_ld32(u);
-            }
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = tiles[i] > 0 ? __uint_as_float(u[x]) : 0.0f;
-            if (s_poison && mine) {
-                for (int pos = guarded * kPromptKeys; pos < sees; ++pos) {
-                    const long long row = cache_row(p.cache, it.seq, pos, it.head);
-                    if (row < 0) continue;
-                    const T *v = static_cast<const T *>(p.cache.v) + row + 32 * q;
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        const float f = static_cast<float>(v[x]);
-                        if (!isfinite(f)) o[x] += f;
-                    }
-                }
-            }
-            if (mine) {
-#pragma unroll
-                for (int x = 0; x < 32; x += 8) {
-                    float y[8];
-#pragma unroll
-                    for (int z = 0; z < 8; ++z) y[z] = o[x + z] * inv;
-                    *reinterpret_cast<uint4 *>(out + 32 * q + x) =
-                        make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
-                }
-            }
-        }
-        tc_fence_before();
     }
+    tc_fence_before();
     __syncthreads();
     if (warp == 8) {
         tc_fence_after();
