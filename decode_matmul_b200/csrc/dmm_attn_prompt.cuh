@@ -34,6 +34,8 @@ struct PromptParams {
 
 constexpr int kPromptThreads = 384;
 constexpr int kPromptKeys = 128;  // keys of a tile
+constexpr int kPromptEarly = 6;   // of the 8 steps of 16 keys that P V takes: those that begin before the rest of P is there
+constexpr int kPromptPoly = 0;    // one exponential in so many is worked out on the multiply-add units
 
 // Key tiles in which rows of a pair of tiles end: they are 256 tokens at most.
 constexpr int kMostGuarded = 3;
@@ -50,7 +52,7 @@ struct PromptPlan {
     // Barriers, in the order of their use for an item.  What not every item uses twice in a row has a phase of its own, which its users
     // count; the guard's come in two sets that the items use in turn.
     static constexpr int kBarItem = 0, kBarItemFree = 2, kBarNext = 4, kBarQ = 5, kBarQFree = 7, kBarFull = 9, kBarEmpty = kBarFull + kStages,
-                         kBarS = kBarEmpty + kStages, kBarP = kBarS + 2, kBarO = kBarP + 2, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
+                         kBarS = kBarEmpty + kStages, kBarP = kBarS + 2, kBarO = kBarP + 4, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
                          kBarGuard = kBarLook + 2 * kMostGuarded, kNumBars = kBarGuard + 2 * kMostGuarded;
     __device__ static constexpr int phase_bit(int item, int tile) { return (item & 1) * kMostGuarded + tile; }
     __device__ static constexpr int look(int item, int tile) { return kBarLook + phase_bit(item, tile); }
@@ -192,6 +194,140 @@ struct F16Kind<__nv_bfloat16> {
     static constexpr uint32_t kType = (1u << 7) | (1u << 10), kExponent = 0x7F80u;
 };
 
+// 32 columns of 16 rows, as a warp holds an accumulator of 16 x 8 tiles: u[4 c + x] is row lane / 4 (x < 2) or lane / 4 + 8, column
+// 8 c + 2 (lane % 4) + x % 2.
+__device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&u)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Of four lanes, lane q has words (q, 0..3) of a 4 x 4 matrix and gets (0..3, q).
+__device__ __forceinline__ uint4 transposed4(const uint32_t (&w)[4]) {
+    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? w[2] : w[3], 1);
+    const uint32_t a0 = odd ? r0 : w[0], a1 = odd ? w[1] : r0, a2 = odd ? r1 : w[2], a3 = odd ? w[3] : r1;
+    const uint32_t s0 = __shfl_xor_sync(0xffffffffu, upper ? a0 : a2, 2), s1 = __shfl_xor_sync(0xffffffffu, upper ? a1 : a3, 2);
+    return upper ? make_uint4(s0, s1, a2, a3) : make_uint4(a0, a1, s0, s1);
+}
+
+// 2^y on the multiply-add units, for both halves of y (Cody and Waite's reduction: y = n + f with n whole and |f| <= 1/2; a
+// polynomial for 2^f, of the least largest relative error; n into the exponent).  y is at most 64 or so, and what is
+// below -126 counts as -126.  The polynomial is off by 2.6e-6, less than a hundredth of half a step of fp16, or 7.5e-5, a
+// fiftieth of half a step of bf16.
+template <class T>
+__device__ __forceinline__ float2 exp2_poly(float2 y) {
+    const auto both = [](float x) { return pair32(x, x); };
+    const uint64_t yy = pair32(fmaxf(y.x, -126.0f), fmaxf(y.y, -126.0f));
+    const uint64_t t = add2(yy, both(12582912.0f));  // 1.5 * 2^23: the whole part ends in the low bits
+    const uint64_t f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), yy);
+    uint64_t r;
+    if constexpr (F16Kind<T>::kType == 0) {
+        r = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+        r = fma2(r, f, both(0.240247443318367f));
+        r = fma2(r, f, both(0.6931217908859253f));
+        r = fma2(r, f, both(0.9999992847442627f));
+    } else {
+        r = fma2(both(0.0551716685295105f), f, both(0.2426111251115799f));
+        r = fma2(r, f, both(0.6932609677314758f));
+        r = fma2(r, f, both(0.9999280571937561f));
+    }
+    const float2 v = unpair32(r), n = unpair32(t);
+    return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// A thread's row of one tile of scores becomes a row of weights, in tensor memory.  m: the maximum that the weights are taken against,
+// l: their sum so far.
+template <class T, int D>
+struct SoftmaxRow {
+    uint32_t s_at, o_at;   // tensor memory of S (then P) and O
+    float c, turn;         // weights are 2^(c turn S - c m)
+    uint32_t bar;          // barriers of the two parts of P
+    int sees;              // keys of the tile that the row sees
+    bool begun;            // O has a sum already
+
+    // kAny: some row does not see all keys, or the scale is not positive
+    template <bool kAny>
+    __device__ __forceinline__ void step(float &m, float &l) const {
+        uint32_t u[128];
+        tmem_ld32(s_at, u);
+        tmem_ld32(s_at + 32, u + 32);
+        tmem_wait_ld32(u);
+        tmem_wait_ld32(u + 32);
+        tmem_ld32(s_at + 64, u + 64);
+        tmem_ld32(s_at + 96, u + 96);
+        float tops[8];  // (chains of their own)
+        const auto score = [&](int x) { return __uint_as_float(u[x]); };
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (half == 1) {
+                tmem_wait_ld32(u + 64);
+                tmem_wait_ld32(u + 96);
+            }
+            if constexpr (kAny) {
+#pragma unroll
+                for (int x = 64 * half; x < 64 * half + 64; ++x) u[x] = __float_as_uint(x < sees ? score(x) * turn : -INFINITY);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (half == 0) tops[q] = fmaxf(score(q), score(q + 8));
+#pragma unroll
+                for (int x = half == 0 ? 16 : 64; x < 64 * half + 64; x += 16) tops[q] = max3(tops[q], score(x + q), score(x + q + 8));
+            }
+        }
+        const float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
+        const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
+        if (__any_sync(0xffffffffu, rise)) {
+            const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
+            m = to;
+            l *= f;
+            if (begun) {
+#pragma unroll 1
+                for (int q = 0; q < D / 16; ++q) {
+                    uint32_t o[16];
+                    tmem_ld16(o_at + 16 * q, o);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                    tmem_st16(o_at + 16 * q, o);
+                }
+            }
+        }
+        const float mc = m == -INFINITY ? 0.0f : -m * c;
+        const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
+        uint64_t sums[4] = {};
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            uint32_t w[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                float2 y = unpair32(fma2(pair32(score(16 * q + 2 * x), score(16 * q + 2 * x + 1)), c2, mc2));
+                // some on the multiply-add units, which have time to spare (where nothing is hidden: 2^-infinity is 0)
+                if (!kAny && x % 8 >= 8 - kPromptPoly) {
+                    y = exp2_poly<T>(y);
+                } else {
+                    y.x = exp2_fast(y.x);
+                    y.y = exp2_fast(y.y);
+                }
+                sums[x % 4] = add2(sums[x % 4], pair32(y.x, y.y));
+                w[x] = pack16<T>(y.x, y.y);
+            }
+            tmem_st8(s_at + 8 * q, w);
+            if (q + 1 == kPromptEarly || q == 7) {  // the products of these keys can begin
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(bar + (q == 7 ? 8u : 0u));
+            }
+        }
+        const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        l += sum.x + sum.y;
+    }
+};
+
 // The next block of the grid that has not begun, taken over (cluster launch control): asked for, and the answer, -1 when there is none.
 __device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
     fence_async_smem();  // (the answer before has been read)
@@ -240,7 +376,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_failed, s_poison[2];
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tt = p.tile_tokens;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0), lane = threadIdx.x % 32, tt = p.tile_tokens;
     const auto bar = [&](int i) { return smem + Plan::kBars + 8u * static_cast<uint32_t>(i); };
     grid_dep_wait();
     if (warp == 8) {
@@ -255,7 +391,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.
     const auto item_of = [&](int k) {
         mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed);
@@ -269,9 +405,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     };
 
     // Registers: 384 threads are launched with 168 each; the softmax holds a row of 128 scores and wants more, the others need
-    // less (256 * 208 + 128 * 80 = 63488 of 64512).
+    // less (256 * 224 + 128 * 56 = 64512).
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 9) {
             // =============================== items and loads ===============================
             const int shift_pg = p.cache.page_shift, page = 1 << shift_pg, box = min(page, kPromptKeys);
@@ -411,8 +547,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     if (leader) tc_commit(bar(Plan::kBarEmpty + stage));
                     step();
                 }
+                bool v_seen = false, k_seen = false;  // the next values and keys were seen to be there
                 for (int j = 0; j < ext.all; ++j) {
-                    mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
+                    if (!v_seen) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
                     if (j >= ext.guarded) {
                         const int g = j - ext.guarded, at = Plan::phase_bit(k, g);
                         mbar_wait(bar(Plan::guard(k, g)), (guard >> at) & 1u, &s_failed);
@@ -421,9 +558,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const int v_stage = stage;
                     const uint32_t v = lo(place(v_stage), Plan::kHalfBytes);
                     step();
+                    if (j + 1 < ext.all && !k_seen) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
+                    v_seen = k_seen = false;
                     bool k_there = false;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
+                        // (a look at a barrier takes a while even when its phase is complete, and the tensor cores have few products in
+                        // store: the next tiles are looked for before the last products of this round are issued)
+                        if (i == 1 && j + 1 < ext.all) {
+                            const int s1 = stage + 1 == Plan::kStages ? 0 : stage + 1, s2 = s1 + 1 == Plan::kStages ? 0 : s1 + 1;
+                            v_seen = mbar_test(bar(Plan::kBarFull + s1), parity ^ (s1 < stage ? 1u : 0u));
+                            k_seen = j + 2 < ext.all && mbar_test(bar(Plan::kBarFull + s2), parity ^ (s2 < stage ? 1u : 0u));
+                        }
                         if (j < ext.tiles[i]) {
                             if (j == 0) {  // the epilogue before has read O
                                 if (o_used[i]) {
@@ -432,22 +578,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                                 }
                                 o_used[i] = true;
                             }
-                            mbar_wait(bar(Plan::kBarP + i), (p_full >> i) & 1u, &s_failed);
-                            p_full ^= 1u << i;
-                            tc_fence_after();
-                            if (leader) {
-                                // (the last tile: only the 16 keys at a time that some row sees)
-                                const int steps = min(8, (ext.most[i] - j * kPromptKeys + 15) / 16);
-                                for (int n = 0; n < steps; ++n)
-                                    mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * n, v + n * (2048u >> 4), kHi, kIdO, j > 0 || n > 0);
-                                if (j + 1 == ext.tiles[i]) tc_commit(bar(Plan::kBarO + i));
+                            // (the last tile: only the 16 keys at a time that some row sees)
+                            const int steps = min(8, (ext.most[i] - j * kPromptKeys + 15) / 16);
+                            const uint32_t begun = j > 0 ? 1u : 0u;
+#pragma unroll
+                            for (int part = 0; part < 2; ++part) {
+                                mbar_wait(bar(Plan::kBarP + 2 * i + part), (p_full >> i) & 1u, &s_failed);
+                                tc_fence_after();
+                                if (leader) {
+#pragma unroll
+                                    for (int n = part == 0 ? 0 : kPromptEarly; n < (part == 0 ? kPromptEarly : 8); ++n)
+                                        if (n < steps)
+                                            mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * n, v + n * (2048u >> 4), kHi, kIdO, n > 0 ? 1u : begun);
+                                }
+                                __syncwarp();
                             }
-                            __syncwarp();
+                            p_full ^= 1u << i;
+                            if (leader && j + 1 == ext.tiles[i]) tc_commit(bar(Plan::kBarO + i));
                         }
                         if (j + 1 < ext.tiles[i]) {
-                            if (!k_there) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
                             k_there = true;
-                            tc_fence_after();
                             scores(i, stage);
                             if (leader && j + 2 == ext.tiles[i]) tc_commit(bar(Plan::kBarQFree + i));
                         }
@@ -510,9 +660,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // =============================== softmax ===============================
-        const int i = warp / 4, r = threadIdx.x % 128, tok = r / p.group;
+        const int i = warp / 4, r = threadIdx.x % 128, magic = 65536 / p.group + 1, tok = r * magic >> 16;  // (r / group, for r < 128)
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
         const uint32_t s_at = lanes + Plan::kS + 128 * i, o_at = lanes + Plan::kO + D * i;
         // c S <= 0 for c <= 0: such scales turn the sign of S, or make it 0
@@ -533,68 +683,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
                 s_full ^= 1u;
                 tc_fence_after();
-                uint32_t u[128];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, u + 32 * q);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_wait_ld32(u + 32 * q);
-                float s[128];
-#pragma unroll
-                for (int x = 0; x < 128; ++x) s[x] = __uint_as_float(u[x]);
-                if (turn != 1.0f)
-#pragma unroll
-                    for (int x = 0; x < 128; ++x) s[x] *= turn;
-                if (j >= free) {
-                    const int rel = sees - j * kPromptKeys;
-#pragma unroll
-                    for (int x = 0; x < 128; ++x) s[x] = x < rel ? s[x] : -INFINITY;
-                }
-                float tops[4];  // (chains of their own)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tops[q] = fmaxf(s[q], s[q + 4]);
-#pragma unroll
-                    for (int x = 8; x < 128; x += 8) tops[q] = max3(tops[q], s[x + q], s[x + q + 4]);
-                }
-                const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
-                const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
-                if (__any_sync(0xffffffffu, rise)) {
-                    const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
-                    m = to;
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int q = 0; q < D / 16; ++q) {
-                            uint32_t o[16];
-                            tmem_ld16(o_at + 16 * q, o);
-                            tmem_wait_ld(o);
-#pragma unroll
-                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                            tmem_st16(o_at + 16 * q, o);
-                        }
-                    }
-                }
-                const float mc = m == -INFINITY ? 0.0f : -m * c;
-                const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
-                uint64_t sums[4] = {};
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const float2 y = unpair32(fma2(pair32(s[16 * q + 2 * x], s[16 * q + 2 * x + 1]), c2, mc2));
-                        const float a = exp2_fast(y.x), b = exp2_fast(y.y);
-                        sums[x % 4] = add2(sums[x % 4], pair32(a, b));
-                        w[x] = pack16<T>(a, b);
-                    }
-                    tmem_st8(s_at + 8 * q, w);
-                }
-                const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-                l += sum.x + sum.y;
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(Plan::kBarP + i));
+                const SoftmaxRow<T, D> row = {s_at, o_at, c, turn, bar(Plan::kBarP + 2 * i), sees - j * kPromptKeys, j > 0};
+                if (j < free && turn == 1.0f)
+                    row.template step<false>(m, l);
+                else
+                    row.template step<true>(m, l);
             }
             if (tiles > 0) {
                 mbar_wait(bar(Plan::kBarO + i), o_full, &s_failed);
@@ -602,37 +695,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 tc_fence_after();
             }
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + r % p.group) * D;
+            T *const out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + it.token0 + i * tt) * p.out_ld + static_cast<long long>(it.head * p.group) * D;
+            if (s_poison[k & 1]) {
+                // values that are not finite, which the guard has taken out of the tiles in which rows end: row by row
+                T *to = out + static_cast<long long>(tok) * p.out_ld + (r - tok * p.group) * D;
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-                uint32_t u[32];
-                float o[32];
-                if (tiles > 0) {
-                    tmem_ld32(o_at + 32 * q, u);
-                    tmem_wait_ld32(u);
-                }
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = tiles > 0 ? __uint_as_float(u[x]) : 0.0f;
-                if (s_poison[k & 1] && mine) {
+                for (int q = 0; q < D / 16; ++q) {
+                    uint32_t u[16] = {};
+                    if (tiles > 0) {
+                        tmem_ld16(o_at + 16 * q, u);
+                        tmem_wait_ld(u);
+                    }
+                    if (!mine) continue;
+#pragma unroll 1
                     for (int pos = ext.guarded * kPromptKeys; pos < sees; ++pos) {
                         const long long row = cache_row(p.cache, it.seq, pos, it.head);
                         if (row < 0) continue;
-                        const T *v = static_cast<const T *>(p.cache.v) + row + 32 * q;
+                        const T *v = static_cast<const T *>(p.cache.v) + row + 16 * q;
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) {
+                        for (int x = 0; x < 16; ++x) {
                             const float f = static_cast<float>(v[x]);
-                            if (!isfinite(f)) o[x] += f;
+                            if (!isfinite(f)) u[x] = __float_as_uint(__uint_as_float(u[x]) + f);
                         }
                     }
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) to[16 * q + x] = static_cast<T>(__uint_as_float(u[x]) * inv);
                 }
-                if (mine) {
+            } else {
+                // 8 rows of 64 bytes with each store: a row at a time would touch 32 lines
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {  // 8 rows; a fragment has 16
+                    const int rr = 32 * (warp % 4) + 8 * h + lane / 4, t = rr * magic >> 16;
+                    const float f = __shfl_sync(0xffffffffu, inv, 8 * h + lane / 4);
+                    const bool there = t < tt && it.token0 + i * tt + t < it.n;
+                    T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + 8 * (lane % 4);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 8) {
-                        float y[8];
+                    for (int q = 0; q < D / 32; ++q) {
+                        uint32_t u[16] = {}, w[4];
+                        if (tiles > 0) {
+                            tmem_ld16x32(o_at + (static_cast<uint32_t>(h & 2) << 19) + 32 * q, u);
+                            tmem_wait_ld(u);
+                        }
 #pragma unroll
-                        for (int z = 0; z < 8; ++z) y[z] = o[x + z] * inv;
-                        *reinterpret_cast<uint4 *>(out + 32 * q + x) =
-                            make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+                        for (int x = 0; x < 4; ++x) {
+                            const float y0 = __uint_as_float(h & 1 ? u[4 * x + 2] : u[4 * x]), y1 = __uint_as_float(h & 1 ? u[4 * x + 3] : u[4 * x + 1]);
+                            w[x] = pack16<T>(y0 * f, y1 * f);
+                        }
+                        const uint4 piece = transposed4(w);
+                        if (there) *reinterpret_cast<uint4 *>(to + 32 * q) = piece;
                     }
                 }
             }
