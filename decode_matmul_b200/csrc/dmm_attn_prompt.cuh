@@ -626,18 +626,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     look ^= 1u << at;
                     const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>((tile0 + 2 * j + 1) % Plan::kStages) * Plan::kTileBytes;
                     const auto where = [&](int c) { return base + (c / 1024) * Plan::kHalfBytes + (c % 1024) * 16u; };  // piece c: row (c % 1024) / 8
-                    const auto bad = [](uint32_t w) { return (w & 0xFFFFu & kMask) == (kMask & 0xFFFFu) || (w & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u); };
-                    bool any = false;
+                    // a half is not finite if its exponent is all ones: one more there carries into the sign
+                    constexpr uint32_t kOne = (0x8000u - F16Kind<T>::kExponent) * 0x10001u;
+                    const auto carries = [&](uint32_t w) { return (w & kMask) + kOne; };
+                    uint32_t any = 0;
+#pragma unroll 8
                     for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
-                        const int row = (c % 1024) / 8;
-                        if (row < rows) {
+                        if ((c % 1024) / 8 < rows) {
                             const uint4 w = lds128(where(c));
-                            any |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
-                        } else if (row < ((rows + 15) & ~15)) {
-                            sts128(where(c), make_uint4(0, 0, 0, 0));
+                            any |= carries(w.x) | carries(w.y) | carries(w.z) | carries(w.w);
                         }
                     }
-                    if (any) {
+                    for (int c = 8 * rows + t; c < 8 * ((rows + 15) & ~15); c += 64)
+#pragma unroll
+                        for (int hh = 0; hh < Plan::kHalves; ++hh) sts128(where(c + 1024 * hh), make_uint4(0, 0, 0, 0));
+                    if (any & 0x80008000u) {
                         s_poison[k & 1] = 1;
                         for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
                             if ((c % 1024) / 8 >= rows) continue;
@@ -645,8 +648,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                if ((x[i] & 0xFFFFu & kMask) == (kMask & 0xFFFFu)) x[i] &= 0xFFFF0000u;
-                                if ((x[i] & 0xFFFF0000u & kMask) == (kMask & 0xFFFF0000u)) x[i] &= 0xFFFFu;
+                                const uint32_t bad = carries(x[i]);
+                                x[i] &= (bad & 0x8000u ? 0u : 0xFFFFu) | (bad & 0x80000000u ? 0u : 0xFFFF0000u);
                             }
                             sts128(where(c), make_uint4(x[0], x[1], x[2], x[3]));
                         }
@@ -724,25 +727,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             } else {
                 // 8 rows of 64 bytes with each store: a row at a time would touch 32 lines
 #pragma unroll 1
-                for (int h = 0; h < 4; ++h) {  // 8 rows; a fragment has 16
-                    const int rr = 32 * (warp % 4) + 8 * h + lane / 4, t = rr * magic >> 16;
-                    const float f = __shfl_sync(0xffffffffu, inv, 8 * h + lane / 4);
-                    const bool there = t < tt && it.token0 + i * tt + t < it.n;
-                    T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + 8 * (lane % 4);
+                for (int h = 0; h < 2; ++h) {  // 16 rows
+                    uint32_t u[D / 32][16] = {};
+                    if (tiles > 0) {
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {
-                        uint32_t u[16] = {}, w[4];
-                        if (tiles > 0) {
-                            tmem_ld16x32(o_at + (static_cast<uint32_t>(h & 2) << 19) + 32 * q, u);
-                            tmem_wait_ld(u);
-                        }
+                        for (int q = 0; q < D / 32; ++q) tmem_ld16x32(o_at + (static_cast<uint32_t>(h) << 20) + 32 * q, u[q]);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float y0 = __uint_as_float(h & 1 ? u[4 * x + 2] : u[4 * x]), y1 = __uint_as_float(h & 1 ? u[4 * x + 3] : u[4 * x + 1]);
-                            w[x] = pack16<T>(y0 * f, y1 * f);
+                        for (int q = 0; q < D / 32; ++q) tmem_wait_ld(u[q]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int in_warp = 16 * h + 8 * e + lane / 4, rr = 32 * (warp % 4) + in_warp, t = rr * magic >> 16;
+                        const float f = __shfl_sync(0xffffffffu, inv, in_warp);
+                        const bool there = t < tt && it.token0 + i * tt + t < it.n;
+                        T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + 8 * (lane % 4);
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                w[x] = pack16<T>(__uint_as_float(u[q][4 * x + 2 * e]) * f, __uint_as_float(u[q][4 * x + 2 * e + 1]) * f);
+                            const uint4 piece = transposed4(w);
+                            if (there) *reinterpret_cast<uint4 *>(to + 32 * q) = piece;
                         }
-                        const uint4 piece = transposed4(w);
-                        if (there) *reinterpret_cast<uint4 *>(to + 32 * q) = piece;
                     }
                 }
             }
