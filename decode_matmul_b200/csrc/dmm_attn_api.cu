@@ -150,7 +150,8 @@ size_t dmm_attention_workspace_bytes(int64_t tokens, int num_seqs, int heads, in
     (void)tokens, (void)num_seqs, (void)heads, (void)kv_heads;
     int sms = 0;
     if (device_sms(&sms) != 0 || sms < 1) sms = 256;
-    return decode_workspace(head_dim, sms);
+    const size_t decode = decode_workspace(head_dim, sms), prompt = prompt_workspace(head_dim, sms);
+    return decode > prompt ? decode : prompt;
 }
 
 int dmm_paged_attention(const void *q, int64_t q_ld, int heads, float scale, void *out, int64_t out_ld,
@@ -182,8 +183,11 @@ int dmm_prompt_attention(const void *q, int64_t q_ld, int64_t tokens, int heads,
                          size_t workspace_bytes, unsigned flags, void *stream) {
     if (!cu_seqlens) return DMM_ERR_NULL;
     PromptParams p = {};
-    const int rc = check_attention(q, q_ld, tokens, heads, out, out_ld, cache, &p.cache, workspace, workspace_bytes, flags);
+    int rc = check_attention(q, q_ld, tokens, heads, out, out_ld, cache, &p.cache, workspace, workspace_bytes, flags);
     if (rc) return rc;
+    rc = device_sms(&p.ctas);
+    if (rc) return rc;
+    p.workspace = static_cast<uint8_t *>(workspace);
     p.q = q;
     p.out = out;
     p.cu = cu_seqlens;
@@ -193,7 +197,7 @@ int dmm_prompt_attention(const void *q, int64_t q_ld, int64_t tokens, int heads,
     p.heads = heads;
     p.group = heads / cache->kv_heads;
     p.scale = scale;
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    g_launches.fetch_add(2, std::memory_order_relaxed);
     return launch_prompt(p, cache->type, cache->head_dim, (flags & DMM_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream));
 }
 

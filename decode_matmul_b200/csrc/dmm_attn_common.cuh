@@ -44,6 +44,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ void load_floats(const float *p, float (&x)[4]) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+}
+__device__ __forceinline__ void load_floats(const float *p, float (&x)[2]) {
+    const float2 f = *reinterpret_cast<const float2 *>(p);
+    x[0] = f.x, x[1] = f.y;
+}
+
 // Lets a kernel have more than 48 KB of dynamic shared memory, once per device.
 struct SmemAllowance {
     std::atomic<bool> given[64];

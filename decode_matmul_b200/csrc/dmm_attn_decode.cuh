@@ -189,15 +189,6 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void load_floats(const float *p, float (&x)[4]) {
-    const float4 f = *reinterpret_cast<const float4 *>(p);
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-}
-__device__ __forceinline__ void load_floats(const float *p, float (&x)[2]) {
-    const float2 f = *reinterpret_cast<const float2 *>(p);
-    x[0] = f.x, x[1] = f.y;
-}
-
 // What a warp has of one segment when it could not write it out.
 struct DecodePart {
     long long start;

@@ -30,6 +30,8 @@ struct PromptParams {
     CacheView cache;
     int tokens, heads, group, tile_tokens;  // tile_tokens = 128 / group: tokens of a tile
     float scale;
+    uint8_t *workspace;  // see PromptHead
+    int ctas;
 };
 
 constexpr int kPromptThreads = 384;
@@ -145,43 +147,162 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-// What a CTA works on.
+// What a CTA works on: a pair of tiles of one key head, or a part of its key tiles.
 struct PromptItem {
     int seq, head, begin, n, len, token0;  // token0: first token of tile 0 within the sequence's new tokens
+    int first, end;                        // key tiles
+    int slot;                              // of the workspace, for a part; -1 for the whole
+    int ctas;                              // for the first part: how many CTAs have one
 };
 
-// Item `index` in the order: sequences as they come, tile pairs from the last (which has the most keys) to the first,
-// key heads innermost.  By the lanes of one warp; seq = -1 when there is no such item.
-__device__ __forceinline__ PromptItem prompt_item(const PromptParams &p, int index) {
-    const int lane = threadIdx.x & 31, span_tokens = 2 * p.tile_tokens;
-    PromptItem it = {-1, index % p.cache.kv_heads, 0, 0, 0, 0};
-    int rest = index / p.cache.kv_heads;
-    for (int b0 = 0; b0 < p.cache.num_seqs; b0 += 32) {
-        const int b = b0 + lane;
-        TokenSpan s = {0, 0};
-        if (b < p.cache.num_seqs) s = token_span(p.cu, b, p.tokens);
-        const int pairs = (s.n + span_tokens - 1) / span_tokens;
-        int upto = pairs;
+constexpr int kPromptItem = 2;
+constexpr float kPromptJoin = 4.0f;
+
+// The sequences of one lane each, from b0 on; by a warp.
+struct PromptSeqs {
+    TokenSpan span;
+    int len, pairs, first, last;  // first, last: key tiles of the first pair of tiles, and of the last
+    __device__ __forceinline__ int units() const { return last + kPromptItem; }
+    __device__ __forceinline__ PromptSeqs(const PromptParams &p, int b0) {
+        const int b = b0 + static_cast<int>(threadIdx.x & 31);
+        span = {0, 0};
+        len = 0;
+        if (b < p.cache.num_seqs) span = token_span(p.cu, b, p.tokens);
+        if (span.n > 0) len = cache_len(p.cache, b);
+        pairs = (span.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+        first = span.n > 0 ? (max(0, len - span.n + min(2 * p.tile_tokens, span.n)) + kPromptKeys - 1) / kPromptKeys : 0;
+        last = span.n > 0 ? (len + kPromptKeys - 1) / kPromptKeys : 0;
+    }
+};
+__device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// How the work is shared out: the same in every CTA, by a warp.
+//   each == 0   whole items, which the CTAs take as they come, those with the most keys first.  A prompt from its beginning has items
+//               of every length, and the short ones fill up what the long ones leave.
+//   otherwise   the key tiles of all items in one line, cut into even shares: CTA x has units [begin(x), begin(x + 1)).  For few
+//               items or long ones of one length (the next chunk of a prompt), which would leave CTAs idle.  An item counts as
+//               many units as the last of its sequence has key tiles, and kPromptItem more for its beginning and end.  What CTAs
+//               have of an item that they share goes through the workspace to a second kernel, which takes as long as
+//               kPromptJoin key tiles.
+// Which of the two ends sooner is estimated: whole items end with the longest, or half of the shortest of a sequence (on
+// average over the work) behind an even share.
+struct PromptShare {
+    int each, more;
+    __device__ __forceinline__ int begin(int x) const { return each * x + min(x, more); }
+    __device__ __forceinline__ int owner(int u) const { return u < (each + 1) * more ? u / (each + 1) : more + (u - (each + 1) * more) / each; }
+};
+// `first`: the sequences from 0 on
+__device__ __forceinline__ PromptShare prompt_share(const PromptParams &p, const PromptSeqs &first) {
+    float items = 0.0f, tiles = 0.0f, units = 0.0f, least = 0.0f;
+    int longest = 0;
+    PromptSeqs q = first;
+    for (int b0 = 0;;) {
+        const float n = static_cast<float>(q.pairs) * static_cast<float>(p.cache.kv_heads), mean = 0.5f * static_cast<float>(q.first + q.last) + kPromptItem;
+        items += n;
+        tiles += n * mean;
+        units += n * static_cast<float>(q.units());
+        least += n * mean * static_cast<float>(q.first);
+        longest = max(longest, q.last);
+        b0 += 32;
+        if (b0 >= p.cache.num_seqs) break;
+        q = PromptSeqs(p, b0);
+    }
+    items = warp_sum(items), tiles = warp_sum(tiles), units = warp_sum(units), least = warp_sum(least);
+    const float ctas = static_cast<float>(p.ctas), most = static_cast<float>(__reduce_max_sync(0xffffffffu, longest));
+    const float whole = items <= ctas ? most : fmaxf(most, tiles / ctas + 0.5f * least / fmaxf(tiles, 1.0f));
+    if (units > 1e9f || whole <= units / ctas + kPromptJoin) return {0, 0};
+    int all = 0;
+    q = first;
+    for (int b0 = 0;;) {
+        all += q.pairs * p.cache.kv_heads * q.units();
+        b0 += 32;
+        if (b0 >= p.cache.num_seqs) break;
+        q = PromptSeqs(p, b0);
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    const int each = all / p.ctas;
+    return {each, all - each * p.ctas};  // (each > 0: whole items are as good where there are fewer units than CTAs)
+}
+
+// 32 sequences in the order of the work: those with the longest contexts first, so that what begins late is short.  A lane's sequence
+// has `mine` items or units, behind `before` of others.
+struct PromptLine {
+    PromptSeqs q;
+    int size, mine, before;  // size: units of an item
+    __device__ __forceinline__ PromptLine(const PromptParams &p, const PromptShare &share, const PromptSeqs &seqs, int b0) : q(seqs) {
+        const int lane = threadIdx.x & 31, there = min(32, p.cache.num_seqs - b0);
+        size = share.each > 0 ? q.units() : 1;
+        mine = q.pairs * p.cache.kv_heads * size;
+        before = 0;
+        for (int l = 0; l < there; ++l) {
+            const int other = __shfl_sync(0xffffffffu, q.last, l), theirs = __shfl_sync(0xffffffffu, mine, l);
+            if (other > q.last || (other == q.last && l < lane)) before += theirs;
         }
-        const unsigned after = __ballot_sync(0xffffffffu, upto > rest);
-        if (after != 0) {
-            const int who = __ffs(after) - 1;
-            it.seq = b0 + who;
-            it.begin = __shfl_sync(0xffffffffu, s.begin, who);
-            it.n = __shfl_sync(0xffffffffu, s.n, who);
-            const int at = rest - __shfl_sync(0xffffffffu, upto - pairs, who);
-            it.token0 = (__shfl_sync(0xffffffffu, pairs, who) - 1 - at) * span_tokens;
-            it.len = cache_len(p.cache, it.seq);
-            return it;
+    }
+};
+
+// Item `index`, or the item of unit `index`, of which [index, end) is wanted; the order: 32 sequences at a time, tile pairs from the last
+// (which has the most keys) to the first, key heads innermost.  By a warp; seq = -1 when there is no such item.  `first`: the
+// sequences from 0 on.  *upto: the first unit behind what the item covers of [index, end).
+__device__ __forceinline__ PromptItem prompt_item(const PromptParams &p, const PromptShare &share, const PromptLine &first, int index, int end, int *upto) {
+    PromptItem it = {-1, 0, 0, 0, 0, 0, 0, 0, -1, 0};
+    int rest = index, b0 = 0;
+    PromptLine line = first;
+    unsigned here;
+    for (;;) {
+        here = __ballot_sync(0xffffffffu, rest >= line.before && rest - line.before < line.mine);
+        if (here != 0) break;
+        rest -= __reduce_add_sync(0xffffffffu, line.mine);
+        b0 += 32;
+        if (b0 >= p.cache.num_seqs) return it;
+        line = PromptLine(p, share, PromptSeqs(p, b0), b0);
+    }
+    const int who = __ffs(here) - 1, at = __shfl_sync(0xffffffffu, rest - line.before, who);
+    it.seq = b0 + who;
+    it.begin = __shfl_sync(0xffffffffu, line.q.span.begin, who);
+    it.n = __shfl_sync(0xffffffffu, line.q.span.n, who);
+    it.len = __shfl_sync(0xffffffffu, line.q.len, who);
+    const int pairs = __shfl_sync(0xffffffffu, line.q.pairs, who);
+    int item = at, units = 1, unit = 0;
+    if (share.each > 0) {
+        units = __shfl_sync(0xffffffffu, line.size, who);
+        item = at / units;
+        unit = at - item * units;
+    }
+    const int nth = item / p.cache.kv_heads;
+    it.head = item - nth * p.cache.kv_heads;
+    it.token0 = (pairs - 1 - nth) * 2 * p.tile_tokens;
+    it.end = (max(0, it.len - it.n + min(it.token0 + 2 * p.tile_tokens, it.n)) + kPromptKeys - 1) / kPromptKeys;
+    if (share.each > 0) {
+        const int take = min(units - unit, end - index);
+        *upto = index + take;
+        if (take < units) {
+            const int all = it.end;
+            it.first = static_cast<int>(static_cast<long long>(all) * unit / units);
+            it.end = static_cast<int>(static_cast<long long>(all) * (unit + take) / units);
+            const int x = share.owner(index);
+            it.slot = 2 * x + (unit == 0 ? 1 : 0);  // a CTA has at most one item that began before it, and one that goes on behind it
+            if (unit == 0) it.ctas = share.owner(index + units - 1) - x + 1;
         }
-        rest -= __shfl_sync(0xffffffffu, upto, 31);
     }
     return it;
 }
+
+// The workspace: whether items are shared; for each CTA the item that begins in it and goes on in others (ctas: how many have a part,
+// 0 = there is none); then two slots for each CTA: weighted sums of values [256][D], maxima and sums [256][2].
+struct PromptHead {
+    int shared, pad[63];
+};
+__host__ __device__ inline size_t prompt_slots_at(int ctas) { return sizeof(PromptHead) + (static_cast<size_t>(ctas) * sizeof(PromptItem) + 255) / 256 * 256; }
+__device__ __forceinline__ PromptItem *prompt_crossings(const PromptParams &p) { return reinterpret_cast<PromptItem *>(p.workspace + sizeof(PromptHead)); }
+__device__ __forceinline__ float *prompt_slot(const PromptParams &p, int head_dim, int slot) {
+    return reinterpret_cast<float *>(p.workspace + prompt_slots_at(p.ctas)) + static_cast<size_t>(slot) * 256 * (head_dim + 2);
+}
+inline size_t prompt_workspace(int head_dim, int ctas) { return prompt_slots_at(ctas) + static_cast<size_t>(ctas) * 2 * 256 * (head_dim + 2) * sizeof(float); }
 
 template <class T>
 struct F16Kind;  // operand type bits of the instruction descriptor; a word whose 16-bit halves are all exponent
@@ -346,8 +467,8 @@ __device__ __forceinline__ int next_block(uint32_t answer) {
     return x;
 }
 
-// What follows from an item: the key tiles of each of its two tiles, how many keys their last rows see, and the first key tile in which
-// a row ends (or the sequence).  Row t of the new tokens sees keys below len - n + t + 1.
+// What follows from an item: its key tiles for each of its two tiles (from `first` on), how many keys their last rows see, and the first
+// key tile in which a row ends (or the sequence).  Row t of the new tokens sees keys below len - n + t + 1.
 struct PromptExtent {
     int tiles[2], most[2], all, guarded;
     __device__ __forceinline__ PromptExtent(const PromptItem &it, int tile_tokens) {
@@ -356,9 +477,9 @@ struct PromptExtent {
         for (int i = 0; i < 2; ++i) {
             const int t0 = it.token0 + i * tile_tokens, t1 = min(t0 + tile_tokens, it.n);
             most[i] = t1 > t0 ? max(0, shift + t1 - 1) : 0;
-            tiles[i] = (most[i] + kPromptKeys - 1) / kPromptKeys;
+            tiles[i] = max(0, min(it.end, (most[i] + kPromptKeys - 1) / kPromptKeys) - it.first);
         }
-        all = max(tiles[0], tiles[1]);
+        all = it.end - it.first;
         guarded = max(0, shift + it.token0) / kPromptKeys;
     }
 };
@@ -392,6 +513,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    grid_dep_launch();  // (the kernel that joins parts waits for this one's end)
     // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.
     const auto item_of = [&](int k) {
         mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed);
@@ -405,18 +527,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     };
 
     // Registers: 384 threads are launched with 168 each; the softmax holds a row of 128 scores and wants more, the others need
-    // less (256 * 224 + 128 * 56 = 64512).
+    // less (256 * 216 + 128 * 72 = 64512).
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 9) {
             // =============================== items and loads ===============================
             const int shift_pg = p.cache.page_shift, page = 1 << shift_pg, box = min(page, kPromptKeys);
             int index = static_cast<int>(blockIdx.x), stage = 0;
-            uint32_t parity = 1, q_free = 0;  // q_free: bits, phases
+            uint32_t parity = 1, q_free = 0, asked = 0;  // q_free: bits, phases
             bool q_used[2] = {false, false};
+            const PromptSeqs seqs(p, 0);
+            const PromptShare share = prompt_share(p, seqs);
+            const PromptLine line(p, share, seqs, 0);
+            const bool shared = share.each > 0;
+            int unit = 0, unit_end = 0;  // of an even share: what is left of it
+            PromptItem crossing = {-1, 0, 0, 0, 0, 0, 0, 0, -1, 0};
+            const auto begin_block = [&]() {  // block `index` is this CTA's
+                if (index == 0 && lane == 0) reinterpret_cast<PromptHead *>(p.workspace)->shared = shared;
+                if (!shared || index < 0 || index >= p.ctas) return;
+                unit = share.begin(index);
+                unit_end = share.begin(index + 1);
+            };
+            const auto ask = [&]() {
+                if (lane == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
+                __syncwarp();
+            };
+            const auto answer = [&]() {
+                mbar_wait(bar(Plan::kBarNext), asked & 1u, &s_failed);
+                ++asked;
+                index = next_block(smem_u32(s_answer));
+                __syncwarp();
+                begin_block();
+            };
+            begin_block();
             for (int k = 0;; ++k) {
-                PromptItem it = {-1, 0, 0, 0, 0, 0};
-                if (index >= 0) it = prompt_item(p, index);
+                PromptItem it = {-1, 0, 0, 0, 0, 0, 0, 0, -1, 0};
+                bool more = false;  // of this block's share
+                while (index >= 0) {
+                    if (!shared || index < p.ctas) it = prompt_item(p, share, line, shared ? unit : index, unit_end, &unit);
+                    if (it.seq >= 0 || s_failed) break;
+                    ask();  // (the grid has some blocks more than there is work for)
+                    answer();
+                }
+                if (shared && it.seq >= 0) {
+                    more = unit < unit_end;
+                    if (it.ctas > 0) crossing = it;
+                    if (!more && lane == 0) prompt_crossings(p)[index] = crossing;
+                    if (!more) crossing.ctas = 0;
+                }
                 if (k >= 2) mbar_wait(bar(Plan::kBarItemFree + (k & 1)), static_cast<uint32_t>((k >> 1) - 1) & 1u, &s_failed);
                 if (s_failed) it.seq = -1;
                 if (lane == 0) {
@@ -424,17 +582,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     s_poison[k & 1] = 0;
                     mbar_arrive(bar(Plan::kBarItem + (k & 1)));
                 }
-                if (it.seq < 0) {
-                    // blocks behind the last item need not begin at all
-                    for (; index >= 0 && !s_failed; ++k) {
-                        if (lane == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
-                        __syncwarp();
-                        mbar_wait(bar(Plan::kBarNext), static_cast<uint32_t>(k) & 1u, &s_failed);
-                        index = next_block(smem_u32(s_answer));
-                        __syncwarp();
-                    }
-                    break;
-                }
+                if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -453,10 +601,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                 }
                 const int32_t *table = p.cache.page_table + it.seq * p.cache.table_stride;
-                if (lane == 0 && ext.all == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
+                if (ext.all == 0 && !more) ask();
                 for (int j = 0; j < ext.all; ++j) {
-                    if (lane == 0 && j + 1 == ext.all) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
-                    const int pos = j * kPromptKeys + lane * box;
+                    if (j + 1 == ext.all && !more) ask();
+                    const int tile = it.first + j, pos = tile * kPromptKeys + lane * box;
                     const bool mine = lane * box < kPromptKeys && pos < it.len;
                     int pg = 0;
                     if (mine) {
@@ -472,7 +620,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         mbar_wait(bar(Plan::kBarEmpty + stage), parity, &s_failed);
                         if (s_failed) break;
                         // (values that the guard looks at first arrive at barriers of their own)
-                        const uint32_t full = bar(kv == 1 && j >= ext.guarded ? Plan::look(k, j - ext.guarded) : Plan::kBarFull + stage);
+                        const uint32_t full = bar(kv == 1 && tile >= ext.guarded ? Plan::look(k, tile - ext.guarded) : Plan::kBarFull + stage);
                         if (lane == 0) mbar_arrive_expect_tx(full, bytes);
                         __syncwarp();
                         if (mine) {
@@ -481,16 +629,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             for (int hh = 0; hh < Plan::kHalves; ++hh)
                                 tma_load_4d(dst + hh * Plan::kHalfBytes, kv == 0 ? &kmap : &vmap, 64 * hh, pos & (page - 1), it.head, pg, full);
                         }
-                        if (kv == 1 && j >= ext.guarded && lane == 0) mbar_arrive(bar(Plan::kBarFull + stage));  // (keeps its phases in step)
+                        if (kv == 1 && tile >= ext.guarded && lane == 0) mbar_arrive(bar(Plan::kBarFull + stage));  // (keeps its phases in step)
                         if (++stage == Plan::kStages) {
                             stage = 0;
                             parity ^= 1u;
                         }
                     }
                 }
-                mbar_wait(bar(Plan::kBarNext), static_cast<uint32_t>(k) & 1u, &s_failed);
-                index = next_block(smem_u32(s_answer));
-                __syncwarp();
+                if (more) continue;
+                answer();
             }
             if (s_failed) {  // a wait gave up: copies in flight land before the CTA goes (they take microseconds)
                 const long long t0 = clock64();
@@ -550,8 +697,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 bool v_seen = false, k_seen = false;  // the next values and keys were seen to be there
                 for (int j = 0; j < ext.all; ++j) {
                     if (!v_seen) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
-                    if (j >= ext.guarded) {
-                        const int g = j - ext.guarded, at = Plan::phase_bit(k, g);
+                    if (it.first + j >= ext.guarded) {
+                        const int g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
                         mbar_wait(bar(Plan::guard(k, g)), (guard >> at) & 1u, &s_failed);
                         guard ^= 1u << at;
                     }
@@ -579,7 +726,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                                 o_used[i] = true;
                             }
                             // (the last tile: only the 16 keys at a time that some row sees)
-                            const int steps = min(8, (ext.most[i] - j * kPromptKeys + 15) / 16);
+                            const int steps = min(8, (ext.most[i] - (it.first + j) * kPromptKeys + 15) / 16);
                             const uint32_t begun = j > 0 ? 1u : 0u;
 #pragma unroll
                             for (int part = 0; part < 2; ++part) {
@@ -620,8 +767,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const PromptItem it = item_of(k);
                 if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
-                for (int j = ext.guarded; j < ext.all; ++j) {
-                    const int rows = min(kPromptKeys, it.len - j * kPromptKeys), g = j - ext.guarded, at = Plan::phase_bit(k, g);
+                for (int j = max(0, ext.guarded - it.first); j < ext.all; ++j) {
+                    const int rows = min(kPromptKeys, it.len - (it.first + j) * kPromptKeys), g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
                     mbar_wait(bar(Plan::look(k, g)), (look >> at) & 1u, &s_failed);
                     look ^= 1u << at;
                     const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>((tile0 + 2 * j + 1) % Plan::kStages) * Plan::kTileBytes;
@@ -663,7 +810,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // =============================== softmax ===============================
         const int i = warp / 4, r = threadIdx.x % 128, magic = 65536 / p.group + 1, tok = r * magic >> 16;  // (r / group, for r < 128)
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
@@ -680,13 +827,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int token = it.token0 + i * tt + tok, shift = it.len - it.n + 1;
             const bool mine = tok < tt && token < it.n;
             const int sees = mine ? max(0, shift + token) : 0;
-            const int free = max(0, shift + it.token0 + i * tt) / kPromptKeys;  // key tiles that every row of this tile sees whole
+            const int free = max(0, shift + it.token0 + i * tt) / kPromptKeys - it.first;  // key tiles that every row of this tile sees whole
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < tiles; ++j) {
                 mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
                 s_full ^= 1u;
                 tc_fence_after();
-                const SoftmaxRow<T, D> row = {s_at, o_at, c, turn, bar(Plan::kBarP + 2 * i), sees - j * kPromptKeys, j > 0};
+                const SoftmaxRow<T, D> row = {s_at, o_at, c, turn, bar(Plan::kBarP + 2 * i), sees - (it.first + j) * kPromptKeys, j > 0};
                 if (j < free && turn == 1.0f)
                     row.template step<false>(m, l);
                 else
@@ -697,7 +844,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 o_full ^= 1u;
                 tc_fence_after();
             }
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const bool part = it.slot >= 0;
+            const float inv = part ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            float *const share = part ? prompt_slot(p, D, it.slot) + 128 * D * i : nullptr;
+            if (part) *reinterpret_cast<float2 *>(prompt_slot(p, D, it.slot) + 256 * D + 2 * (128 * i + r)) = make_float2(m == -INFINITY ? m : m * c, l);
             T *const out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + it.token0 + i * tt) * p.out_ld + static_cast<long long>(it.head * p.group) * D;
             if (s_poison[k & 1]) {
                 // values that are not finite, which the guard has taken out of the tiles in which rows end: row by row
@@ -711,7 +861,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                     if (!mine) continue;
 #pragma unroll 1
-                    for (int pos = ext.guarded * kPromptKeys; pos < sees; ++pos) {
+                    for (int pos = max(ext.guarded, it.first) * kPromptKeys; pos < min(sees, it.end * kPromptKeys); ++pos) {
                         const long long row = cache_row(p.cache, it.seq, pos, it.head);
                         if (row < 0) continue;
                         const T *v = static_cast<const T *>(p.cache.v) + row + 16 * q;
@@ -722,7 +872,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         }
                     }
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) to[16 * q + x] = static_cast<T>(__uint_as_float(u[x]) * inv);
+                    for (int x = 0; x < 16; ++x) {
+                        if (part)
+                            share[r * D + 16 * q + x] = __uint_as_float(u[x]);
+                        else
+                            to[16 * q + x] = static_cast<T>(__uint_as_float(u[x]) * inv);
+                    }
                 }
             } else {
                 // 8 rows of 64 bytes with each store: a row at a time would touch 32 lines
@@ -741,6 +896,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         const float f = __shfl_sync(0xffffffffu, inv, in_warp);
                         const bool there = t < tt && it.token0 + i * tt + t < it.n;
                         T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + 8 * (lane % 4);
+                        if (part) {
+                            if (tiles > 0 && there)
+#pragma unroll
+                                for (int q = 0; q < D / 32; ++q)
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x)
+                                        *reinterpret_cast<uint2 *>(share + rr * D + 32 * q + 8 * x + 2 * (lane % 4)) = make_uint2(u[q][4 * x + 2 * e], u[q][4 * x + 2 * e + 1]);
+                            continue;
+                        }
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) {
                             uint32_t w[4];
@@ -764,6 +928,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins what several CTAs have of an item.  Block x has the item that begins in CTA x.
+template <class T, int D>
+__global__ void __launch_bounds__(1024) prompt_join_kernel(const PromptParams p) {
+    grid_dep_wait();
+    if (reinterpret_cast<const PromptHead *>(p.workspace)->shared == 0) return;
+    const PromptItem it = prompt_crossings(p)[blockIdx.x];
+    if (it.ctas == 0) return;
+    const auto slot = [&](int s) { return prompt_slot(p, D, s == 0 ? it.slot : 2 * (static_cast<int>(blockIdx.x) + s)); };
+    constexpr int kPieces = D / 32;  // of four columns, 32 columns apart
+    // eight lanes have a row
+    for (int row = threadIdx.x / 8; row < 256; row += 128) {
+        const int lane = threadIdx.x % 8, tok = row % 128 / p.group, token = it.token0 + row / 128 * p.tile_tokens + tok;
+        if (tok >= p.tile_tokens || token >= it.n) continue;
+        float top = -INFINITY, sum = 0.0f, acc[kPieces][4] = {};
+#pragma unroll 2
+        for (int s = 0; s < it.ctas; ++s) {
+            const float2 ml = *reinterpret_cast<const float2 *>(slot(s) + 256 * D + 2 * row);
+            if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part whose keys the row does not see: it has no sums
+            float f[kPieces][4];
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) load_floats(slot(s) + row * D + 32 * q + 4 * lane, f[q]);
+            const float to = fmaxf(top, ml.x), old = top == -INFINITY ? 0.0f : exp2_fast(top - to), w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - to);
+            top = to;
+            sum = sum * old + w * ml.y;
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[q][x] = acc[q][x] * old + w * f[q][x];
+        }
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + row % 128 - tok * p.group) * D + 4 * lane;
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q)
+            *reinterpret_cast<uint2 *>(out + 32 * q) = make_uint2(pack16<T>(acc[q][0] * inv, acc[q][1] * inv), pack16<T>(acc[q][2] * inv, acc[q][3] * inv));
     }
 }
 
@@ -804,13 +1005,13 @@ inline int launch_prompt_typed(PromptParams &p, int type, bool pdl, cudaStream_t
     }
     // every sequence adds at most one pair of tiles that is not full
     const long long items = (p.tokens / (2 * p.tile_tokens) + static_cast<long long>(p.cache.num_seqs < p.tokens ? p.cache.num_seqs : p.tokens)) * p.cache.kv_heads;
-    if (items > 0x7fffffff) return DMM_ERR_SHAPE;
+    if (items > 0x3fffffff) return DMM_ERR_SHAPE;
     const auto kernel = prompt_attention_kernel<T, D>;
     static SmemAllowance allowance;
     const int rc = allowance.get(reinterpret_cast<const void *>(kernel), Plan::kBytes);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(items));
+    cfg.gridDim = dim3(static_cast<unsigned>(items > p.ctas ? items : p.ctas));  // (even shares: a block for each CTA)
     cfg.blockDim = dim3(kPromptThreads);
     cfg.dynamicSmemBytes = Plan::kBytes;
     cfg.stream = stream;
@@ -819,7 +1020,13 @@ inline int launch_prompt_typed(PromptParams &p, int type, bool pdl, cudaStream_t
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
+    if (err != cudaSuccess) return err;
+    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prompt_join_kernel<T, D>, p);
 }
 
 inline int launch_prompt(PromptParams &p, int type, int head_dim, bool pdl, cudaStream_t stream) {
