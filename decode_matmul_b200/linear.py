@@ -59,8 +59,10 @@ class LinearStack:
     """The linear layers of ``layers`` transformer blocks with synthetic (seeded) codes.
 
     Data flow of one step for a [B, hidden] fp32 residual stream h:
-        a = qkv(fp16(h));  h += o(fp16(a[:, :hidden]))          (attention itself is not part of
-        g = gate_up(fp16(h));  h += down(fp16(silu(g0) * g1))    the operator: q stands in for it)
+        a = qkv(fp16(h));  h += o(fp16(a[:, :hidden]))           (without a cache q stands in for the attention's
+        g = gate_up(fp16(h));  h += down(fp16(silu(g0) * g1))     result: what the products alone take)
+    With a :class:`PagedCache` the rows of h are new tokens of its sequences: a's queries and keys are rotated, its keys and
+    values go into the cache, and o reads the attention's result (:meth:`step`).
     Row-parallel outputs are summed over the tensor-parallel group before the residual add.
     By default the weights are generated directly in sharded form: rank r of w draws its own codes,
     so that no rank ever materialises a full matrix (what the benchmark needs at 17 GB).  With
@@ -121,8 +123,13 @@ class LinearStack:
         # beats a software barrier between resident CTAs
         self.chain_blocks = 0
 
-    def step(self, h: torch.Tensor, path: int = _lib.PATH_AUTO, fused: bool | None = None) -> torch.Tensor:
+    def step(self, h: torch.Tensor, path: int = _lib.PATH_AUTO, fused: bool | None = None, cache=None,
+             cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
         """One pass of the stack over the fp32 residual stream ``h`` [B, hidden] (updated in place).
+
+        ``cache`` (a :class:`PagedCache` of this rank's key heads, fp16): the blocks attend.  The rows of ``h`` are the new
+        tokens of its sequences, for which :meth:`PagedCache.extend` has made room; ``cu_seqlens`` is what that returned, None
+        for one token per sequence.
 
         ``fused`` (default: whenever the batch is at most 32): every elementwise step between two
         layers runs inside the matmul kernels -- the loaders read fp32 and round to fp16 or form
@@ -130,6 +137,8 @@ class LinearStack:
         kernel clears the buffer a later kernel accumulates into.  Four launches per block."""
         if fused is None:
             fused = h.shape[0] <= 32 and path == _lib.PATH_AUTO
+        if cache is not None:
+            return self._step_attend(h, cache, cu_seqlens, path, fused and self.world == 1)
         if fused:
             return self._step_fused(h)
         hid_loc = self.hidden // self.world
@@ -142,6 +151,46 @@ class LinearStack:
             g = blk["gate_up"](h.to(torch.float16), path=path)
             act = (torch.nn.functional.silu(g[:, :ffn_loc]) * g[:, ffn_loc:]).to(torch.float16)
             self._row_parallel(blk["down"], act, h, path)
+        return h
+
+    def _attend(self, i: int, a: torch.Tensor, cache, cu_seqlens, pdl: bool) -> torch.Tensor:
+        """Attention of block ``i`` over the result ``a`` of its qkv product: fp16 [B, heads * head_dim]."""
+        from .attention import append_kv, paged_attention, prompt_attention
+
+        view = (cache.k(i), cache.v(i), cache.page_table, cache.seq_lens)
+        q = append_kv(a, *view, self._freqs, cu_seqlens=cu_seqlens, pdl=pdl)
+        out = paged_attention(q, *view, pdl=pdl) if cu_seqlens is None else prompt_attention(q, *view, cu_seqlens, pdl=pdl)
+        return out.view(out.shape[0], -1)
+
+    def _step_attend(self, h: torch.Tensor, cache, cu_seqlens, path: int, fused: bool) -> torch.Tensor:
+        from .attention import rotary_frequencies
+        from .ops import decode_matmul_sequence, fused_op
+
+        head_dim, kv_heads = self.cfg["head_dim"], self.cfg["kv_heads"] // self.world
+        if cache.layers != len(self.layers) or cache.kv_heads != kv_heads or cache.head_dim != head_dim or cache.pages.dtype != torch.float16:
+            raise RuntimeError(f"cache must be fp16, of {len(self.layers)} layers with {kv_heads} key heads of {head_dim}")
+        if getattr(self, "_freqs", None) is None:
+            self._freqs = rotary_frequencies(head_dim, self.cfg.get("rope_base", 10000.0), device=self.device)
+        ffn_loc = self.ffn // self.world
+        if not fused:
+            for i, blk in enumerate(self.layers):
+                a = blk["qkv"](h.to(torch.float16), path=path)
+                self._row_parallel(blk["o"], self._attend(i, a, cache, cu_seqlens, False), h, path)
+                g = blk["gate_up"](h.to(torch.float16), path=path)
+                act = (torch.nn.functional.silu(g[:, :ffn_loc]) * g[:, ffn_loc:]).to(torch.float16)
+                self._row_parallel(blk["down"], act, h, path)
+            return h
+        buf = self._buffers(h.shape[0])
+        a, g, B = buf["a"], buf["g"], h.shape[0]
+        a.zero_()  # (cleared by the gate_up product of every block from then on)
+        for i, blk in enumerate(self.layers):
+            q, o, gu, dn = blk["qkv"], blk["o"], blk["gate_up"], blk["down"]
+            decode_matmul_sequence((fused_op(h, q, a, zero=g),), B, h.device, workspace=buf["ws"])
+            att = self._attend(i, a, cache, cu_seqlens, True)
+            nxt = self.layers[i + 1]["qkv"] if i + 1 < len(self.layers) else None
+            rest = (fused_op(att, o, h, x_kind=_lib.X_F16), fused_op(h, gu, g, zero=a),
+                    fused_op(g, dn, h, x_kind=_lib.X_F32_SILU_MUL, x_gap=ffn_loc))
+            decode_matmul_sequence(rest, B, h.device, next_weights=nxt, workspace=buf["ws"])
         return h
 
     def _buffers(self, batch: int):

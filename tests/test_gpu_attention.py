@@ -175,6 +175,14 @@ PROMPTS = [
     ([1000], [0], 32, 32, 128, 64, FP16, "heads"),
     ([1500], [0], 10, 2, 128, 16, BF16, "rows"),
     ([1 + (7 * i) % 50 for i in range(60)], [(13 * i) % 90 for i in range(60)], 8, 8, 64, 16, FP16, "heads"),
+    # few rows over long contexts: an item of the kernel is shared by several CTAs, or a CTA has parts of several
+    ([3], [20000], 8, 1, 128, 64, FP16, "heads"),
+    ([40, 1, 300, 2], [9000, 12000, 130, 0], 8, 1, 128, 16, BF16, "rows"),
+    ([200], [7777], 4, 4, 64, 128, FP16, "both"),
+    ([50 + i for i in range(40)], [300 * i for i in range(40)], 4, 2, 128, 32, FP16, "heads"),
+    # more items than CTAs, some of them long: what begins last is short
+    ([1100, 5, 700, 64, 1, 333], [0] * 6, 20, 20, 128, 16, BF16, "heads"),
+    ([2300], [0], 64, 8, 64, 64, FP16, "heads"),
 ]
 
 
@@ -221,6 +229,40 @@ def test_values_behind_a_row_do_not_reach_it(value, group):
     got = dmm.prompt_attention(q, k, v, table, lens, cu_of([200]))
     assert check_attention(got[:70], want[:70], bound[:70]) == 70 * 2 * group * 128
     assert not bool(torch.isfinite(got[70:]).any()) or value == -math.inf
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_one_value_that_is_not_finite(value, dtype):
+    """One element of one value: the rows that see it have it in one column, every other value is as without it.  Also where
+    the context is long and several CTAs share an item."""
+    for new, past, at in ((300, 0, 140), (40, 9000, 9020), (40, 9000, 100)):
+        gen = generator(20)
+        T = new + past
+        k, v, table, lens = make_cache(gen, [T], 1, 128, 64, dtype)
+        q = torch.randn((new, 8, 128), generator=gen, device="cuda").to(dtype)
+        want, bound = attention(q, k, v, table, lens, cu_of([new]))
+        v[int(table[0, at // 64]), 0, at % 64, 17] = value
+        got = dmm.prompt_attention(q, k, v, table, lens, cu_of([new]))
+        seen = torch.arange(past, T, device="cuda") >= at
+        assert not bool(torch.isfinite(got[seen][:, :, 17]).any()) and bool(seen.any())
+        got[seen, :, 17] = 0
+        want[seen, :, 17] = 0
+        assert check_attention(got, want, bound) == got.numel()
+
+
+def test_keys_that_are_not_finite_stay_with_their_rows():
+    # a key of -infinity against positive queries has weight 0: the rows that see it are those without it
+    gen = generator(21)
+    k, v, table, lens = make_cache(gen, [150, 40], 2, 64, 16, FP16)
+    q = torch.rand((190, 4, 64), generator=gen, device="cuda").to(FP16) + 0.1
+    k[int(table[0, 2]), :, 5] = -60000.0
+    want, bound = attention(q, k, v, table, lens, cu_of([150, 40]))
+    k[int(table[0, 2]), :, 5] = -math.inf
+    got = dmm.prompt_attention(q, k, v, table, lens, cu_of([150, 40]))
+    assert check_attention(got, want, bound) == got.numel()
+    one = dmm.paged_attention(q[torch.tensor([149, 189], device="cuda")], k, v, table, lens)
+    assert check_attention(one, want[[149, 189]], bound[[149, 189]]) == one.numel()
 
 
 @pytest.mark.parametrize("dtype", [FP16, BF16])
@@ -425,6 +467,12 @@ def test_workspace_of_the_callers():
     want = dmm.paged_attention(q, k, v, table, lens)
     ws = torch.full((max(need, 1),), 255, dtype=torch.uint8, device="cuda")
     assert torch.equal(dmm.paged_attention(q, k, v, table, lens, workspace=ws), want)
+    # of any content, and of either operator: what the last call left in it does not count
+    qp = torch.randn((12, 8, 128), generator=gen, device="cuda").to(FP16)
+    prompt = dmm.prompt_attention(qp, k, v, table, lens, cu_of([10, 2]))
+    for _ in range(3):
+        assert torch.equal(dmm.prompt_attention(qp, k, v, table, lens, cu_of([10, 2]), workspace=ws), prompt)
+        assert torch.equal(dmm.paged_attention(q, k, v, table, lens, workspace=ws), want)
     if need:
         with pytest.raises(RuntimeError, match="workspace"):
             dmm.paged_attention(q, k, v, table, lens, workspace=ws[:need - 1])
