@@ -12,14 +12,12 @@ working as sequences grow.  What the tables say beyond the cache is not followed
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .ops import _on_device_of
 
 _TYPE_16 = {torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
+_pack = _lib.paged_cache.pack
 _TYPE_IN = {torch.float32: _lib.T_F32, **_TYPE_16}
 
 
@@ -72,8 +70,8 @@ def _check_cache(k, v, table, lens):
         _no("k_pages must be a CUDA tensor")
     if v.get_device() != index or table.get_device() != index or lens.get_device() != index:
         _no("v_pages, page_table and seq_lens must be on the device of k_pages")
-    cache = _lib.PagedCacheArg(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), pages, stride[0], stride[1], stride[2],
-                               table_ld if seqs > 1 else max_pages, kind, kv_heads, head_dim, page_size, seqs, max_pages)
+    cache = _pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), pages, stride[0], stride[1], stride[2],
+                  table_ld if seqs > 1 else max_pages, kind, kv_heads, head_dim, page_size, seqs, max_pages)
     return cache, dtype, index, kv_heads, head_dim, seqs
 
 
@@ -140,11 +138,15 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
             _no("output must be [tokens, heads, head_dim]")
     if tokens == 0:
         return output
-    with _on_device_of(k_pages):
-        rc = _lib.lib().dmm_append_kv(qkv.data_ptr(), kind, qkv.stride(0) if tokens > 1 else width, tokens, heads,
-                                      None if freqs is None else freqs.data_ptr(), 1 if interleaved else 0, output.data_ptr(), out_ld,
-                                      ctypes.byref(cache), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-                                      _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index))
+    args = (qkv.data_ptr(), kind, qkv.stride(0) if tokens > 1 else width, tokens, heads, None if freqs is None else freqs.data_ptr(),
+            1 if interleaved else 0, output.data_ptr(), out_ld, cache, None if cu_seqlens is None else cu_seqlens.data_ptr(),
+            _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index))
+    call = _lib.lib().dmm_append_kv
+    if index == torch.cuda.current_device():
+        rc = call(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args)
     if rc:
         _lib.check(rc, "append_kv")
     return output
@@ -178,26 +180,32 @@ def _attend(name, q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, scale, 
         return output
     if scale is None:
         scale = head_dim ** -0.5
-    flags, stream = _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index)
-    L = _lib.lib()
-    with _on_device_of(k_pages):
-        if workspace is None:
-            # scratch of this call's own, of 16-bit values: the caching allocator knows about streams and captured graphs
-            ws_bytes = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
-            workspace = q.new_empty(((ws_bytes + 1) // 2,))
-        elif not isinstance(workspace, torch.Tensor) or workspace.get_device() != index or not workspace.is_contiguous():
-            _no(f"workspace must be a contiguous tensor on device {index}")
-        else:
-            ws_bytes = workspace.numel() * workspace.element_size()
-        if cu_seqlens is None:
-            rc = L.dmm_paged_attention(q.data_ptr(), q_ld, heads, scale, output.data_ptr(), out_ld, ctypes.byref(cache),
-                                       workspace.data_ptr(), ws_bytes, flags, stream)
-        else:
-            rc = L.dmm_prompt_attention(q.data_ptr(), q_ld, tokens, heads, scale, output.data_ptr(), out_ld, ctypes.byref(cache),
-                                        cu_seqlens.data_ptr(), workspace.data_ptr(), ws_bytes, flags, stream)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = _launch(q, q_ld, tokens, heads, scale, output, out_ld, cache, cu_seqlens, workspace, pdl, index, seqs, kv_heads, head_dim)
+    else:
+        rc = _launch(q, q_ld, tokens, heads, scale, output, out_ld, cache, cu_seqlens, workspace, pdl, index, seqs, kv_heads, head_dim)
     if rc:
         _lib.check(rc, name)
     return output
+
+
+def _launch(q, q_ld, tokens, heads, scale, output, out_ld, cache, cu_seqlens, workspace, pdl, index, seqs, kv_heads, head_dim):
+    """Scratch and the call into the library, on the current device."""
+    L = _lib.lib()
+    if workspace is None:
+        # scratch of this call's own, of 16-bit values: the caching allocator knows about streams and captured graphs
+        ws_bytes = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
+        workspace = q.new_empty(((ws_bytes + 1) // 2,))
+    elif not isinstance(workspace, torch.Tensor) or workspace.get_device() != index or not workspace.is_contiguous():
+        _no(f"workspace must be a contiguous tensor on device {index}")
+    else:
+        ws_bytes = workspace.numel() * workspace.element_size()
+    flags, stream = _lib.FLAG_PDL if pdl else 0, torch._C._cuda_getCurrentRawStream(index)
+    if cu_seqlens is None:
+        return L.dmm_paged_attention(q.data_ptr(), q_ld, heads, scale, output.data_ptr(), out_ld, cache, workspace.data_ptr(), ws_bytes, flags, stream)
+    return L.dmm_prompt_attention(q.data_ptr(), q_ld, tokens, heads, scale, output.data_ptr(), out_ld, cache, cu_seqlens.data_ptr(),
+                                  workspace.data_ptr(), ws_bytes, flags, stream)
 
 
 def paged_attention(q, k_pages, v_pages, page_table, seq_lens, scale=None, output=None, *, workspace=None, pdl=False):

@@ -2,6 +2,8 @@
 tensors that pass for CUDA ones and a library that only records its arguments."""
 import contextlib
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -65,6 +67,10 @@ def test_caches_that_no_kernel_reads(kw):
 
 
 # ------------------------------------------------ what reaches the library ------------------------------------------------
+FIELDS = ("k", "v", "page_table", "seq_lens", "num_pages", "page_stride", "head_stride", "row_stride", "table_stride", "type", "kv_heads",
+          "head_dim", "page_size", "num_seqs", "max_pages")
+
+
 class Dev(torch.Tensor):
     """A CPU tensor that says it lives on CUDA device ``index``."""
     index = 0
@@ -91,8 +97,8 @@ def calls(monkeypatch):
             return 1001
 
         def _call(self, name, args):
-            cache = next(a for a in args if isinstance(a, type(ctypes.byref(ctypes.c_int()))))._obj
-            seen.append((name, args, {f: getattr(cache, f) for f, _ in cache._fields_}))
+            cache = next(a for a in args if isinstance(a, bytes))
+            seen.append((name, args, dict(zip(FIELDS, _lib.paged_cache.unpack(cache)))))
             return 0
 
         def dmm_append_kv(self, *a):
@@ -186,7 +192,7 @@ def test_c_entries_refuse_by_status():
         args = dict(k=p, v=p, page_table=p, seq_lens=p, num_pages=4, page_stride=2048, head_stride=1024, row_stride=64, table_stride=3, type=_lib.T_F16,
                     kv_heads=2, head_dim=64, page_size=16, num_seqs=2, max_pages=3)
         args.update(kw)
-        return ctypes.byref(_lib.PagedCacheArg(**args))
+        return _lib.paged_cache.pack(*(args[f] or 0 for f in FIELDS))
 
     def paged(c, q=p, q_ld=256, heads=4, out=p, out_ld=256, ws=p, ws_bytes=0, flags=0):
         return L.dmm_paged_attention(q, q_ld, heads, 1.0, out, out_ld, c, ws, ws_bytes, flags, None)
@@ -212,6 +218,16 @@ def test_c_entries_refuse_by_status():
     assert L.dmm_append_kv(p, 0, 504, 2, 4, None, 0, p, 256, cache(), None, 0, None) == shape
     assert L.dmm_append_kv(None, 0, 512, 2, 4, None, 0, p, 256, cache(), None, 0, None) == null
     assert L.dmm_attention_workspace_bytes(2, 2, 4, 2, 64) > 0
+
+
+def test_the_fields_are_those_of_the_header():
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "dmm.h")).read()
+    body = re.search(r"typedef struct dmm_paged_cache \{(.*?)\} dmm_paged_cache;", header, re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    fields = [(name.strip().lstrip("*"), "P" if "*" in decl + name else "q" if "int64" in decl else "i")
+              for decl, names in re.findall(r"((?:const )?\w+)\s+([^;]+);", body) for name in names.split(",")]
+    assert tuple(n for n, _ in fields) == FIELDS and "".join(t for _, t in fields) == "PPPPqqqqqiiiiii"
+    assert _lib.paged_cache.size == 96
 
 
 def test_rotary_frequencies():
