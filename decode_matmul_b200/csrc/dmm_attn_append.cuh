@@ -52,6 +52,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
     __shared__ float s_cos[D / 2], s_sin[D / 2];
     grid_dep_wait();
     const int t = blockIdx.x;
+    constexpr int kRuns = D / 16;
+    const int units = (p.heads + 2 * p.cache.kv_heads) * kRuns;
+    const TIn *src = static_cast<const TIn *>(p.qkv) + t * p.qkv_ld;
+    // The first values are asked for before it is known where they go, and then always the next ones ahead.
+    float a[8], bb[8];
+    const auto load = [&](int u, float (&lo)[8], float (&hi)[8]) {
+        const int c = u % kRuns;
+        const TIn *from = src + u / kRuns * D;
+        load8(from + (p.interleaved ? 16 * c : 8 * c), lo);
+        load8(from + (p.interleaved ? 16 * c + 8 : D / 2 + 8 * c), hi);
+    };
+    int u = blockIdx.y * kAppendThreads + threadIdx.x;
+    if (u < units) load(u, a, bb);
     const int b = token_sequence<kAppendThreads>(p.cu, p.cache.num_seqs, p.tokens, t, &s_seq);
     if (b < 0) return;
     const TokenSpan span = token_span(p.cu, b, p.tokens);
@@ -66,15 +79,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
     }
     __syncthreads();
     const long long row = cache_row(p.cache, b, pos, 0);
-    constexpr int kRuns = D / 16;
-    const int units = (p.heads + 2 * p.cache.kv_heads) * kRuns;
-    const TIn *src = static_cast<const TIn *>(p.qkv) + t * p.qkv_ld;
-    for (int u = blockIdx.y * kAppendThreads + threadIdx.x; u < units; u += gridDim.y * kAppendThreads) {
+    while (u < units) {
         const int head = u / kRuns, c = u % kRuns;
         const int lo = p.interleaved ? 16 * c : 8 * c, hi = p.interleaved ? 16 * c + 8 : D / 2 + 8 * c;
-        float a[8], bb[8];
-        load8(src + head * D + lo, a);
-        load8(src + head * D + hi, bb);
+        u += gridDim.y * kAppendThreads;
+        float next_a[8], next_bb[8];
+        if (u < units) load(u, next_a, next_bb);
         if (p.freqs != nullptr && head < p.heads + p.cache.kv_heads) {
             const float *cs = s_cos + 8 * c, *sn = s_sin + 8 * c;
             if (p.interleaved) {
@@ -95,17 +105,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
                 }
             }
         }
-        T *dst;
-        if (head < p.heads) {
-            dst = static_cast<T *>(p.q_out) + t * p.q_ld + head * D;
-        } else {
-            if (row < 0) continue;
+        T *dst = static_cast<T *>(p.q_out) + t * p.q_ld + head * D;
+        if (head >= p.heads) {
             const int h = head - p.heads;
             dst = h < p.cache.kv_heads ? static_cast<T *>(p.cache.k) + row + h * p.cache.head_stride
                                        : static_cast<T *>(p.cache.v) + row + (h - p.cache.kv_heads) * p.cache.head_stride;
         }
-        store8(dst + lo, a);
-        store8(dst + hi, bb);
+        if (head < p.heads || row >= 0) {
+            store8(dst + lo, a);
+            store8(dst + hi, bb);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            a[i] = next_a[i];
+            bb[i] = next_bb[i];
+        }
     }
 }
 
