@@ -446,25 +446,41 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         const DecodePart of = s_part[i];
         const bool whole = __reduce_add_sync(0xffffffffu, member ? have : 0) == of.units;
         const int slot = of.start < c0 ? 0 : 1;  // a CTA has at most one segment that began before it, and one that goes on behind it
-        if (!whole && slot == 1) crossing = {of.seq, of.head, of.tile, share.owner(of.start + of.units - 1) - static_cast<int>(blockIdx.x) + 1};
+        if (!whole && slot == 1 && threadIdx.x == 0) crossing = {of.seq, of.head, of.tile, share.owner(of.start + of.units - 1) - static_cast<int>(blockIdx.x) + 1};
         const int rows = min(Plan::kRows, p.group - of.tile * Plan::kRows);
         for (int row = (warp - nth) & (kDecodeWarps - 1); row < rows; row += kDecodeWarps) {
             constexpr int kC = D / 32;  // columns of a lane
-            const float2 ml = member ? *reinterpret_cast<const float2 *>(my_part + Plan::kRows * Plan::kPad + 2 * row) : make_float2(-INFINITY, 0.0f);
+            // (of a segment at most the last part is a first part, which lies in the workspace: its row is asked for first)
+            const unsigned far = members & 0x55555555u;
+            float acc[kC] = {};
+            if (far != 0) load_floats(first_parts + (__ffs(far) - 1) / 2 * Plan::kPartFloats + row * Plan::kPad + kC * lane, acc);
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (member) ml = *reinterpret_cast<const float2 *>(my_part + Plan::kRows * Plan::kPad + 2 * row);
             float top = ml.x;
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+            for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+            top = __shfl_sync(0xffffffffu, top, 0);
             const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
-            float sum = w * ml.y, acc[kC] = {};
+            float sum = w * ml.y;
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-#pragma unroll 1
-            for (unsigned todo = members; todo != 0; todo &= todo - 1) {
+            for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            sum = __shfl_sync(0xffffffffu, sum, 0);
+            const float w_far = far != 0 ? __shfl_sync(0xffffffffu, w, __ffs(far) - 1) : 0.0f;
+#pragma unroll
+            for (int y = 0; y < kC; ++y) acc[y] *= w_far;
+            const uint32_t near = smem_u32(smem_raw) + 4 * (row * Plan::kPad + kC * lane);
+#pragma unroll 2
+            for (unsigned todo = members & 0xAAAAAAAAu; todo != 0; todo &= todo - 1) {
                 const int x = __ffs(todo) - 1;
                 const float wx = __shfl_sync(0xffffffffu, w, x);
                 float from[kC];
-                load_floats((x % 2 == 0 ? static_cast<const float *>(first_parts) + x / 2 * Plan::kPartFloats
-                                        : reinterpret_cast<const float *>(smem_raw + x / 2 * Plan::kWarpBytes)) + row * Plan::kPad + kC * lane, from);
+                if constexpr (kC == 4) {
+                    const uint4 f = lds128(near + x / 2 * Plan::kWarpBytes);
+                    from[0] = __uint_as_float(f.x), from[1] = __uint_as_float(f.y), from[2] = __uint_as_float(f.z), from[3] = __uint_as_float(f.w);
+                } else {
+                    const uint2 f = lds64(near + x / 2 * Plan::kWarpBytes);
+                    from[0] = __uint_as_float(f.x), from[1] = __uint_as_float(f.y);
+                }
 #pragma unroll
                 for (int y = 0; y < kC; ++y) acc[y] += wx * from[y];
             }
