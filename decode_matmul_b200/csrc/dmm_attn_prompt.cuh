@@ -36,8 +36,7 @@ struct PromptParams {
 
 constexpr int kPromptThreads = 384;
 constexpr int kPromptKeys = 128;  // keys of a tile
-constexpr int kPromptEarly = 6;   // of the 8 steps of 16 keys that P V takes: those that begin before the rest of P is there
-constexpr int kPromptPoly = 0;    // one exponential in so many is worked out on the multiply-add units
+constexpr int kPromptEarly = 5;   // of the 8 steps of 16 keys that P V takes: those that begin before the rest of P is there
 
 // Key tiles in which rows of a pair of tiles end: they are 256 tokens at most.
 constexpr int kMostGuarded = 3;
@@ -156,7 +155,7 @@ struct PromptItem {
 };
 
 constexpr int kPromptItem = 2;
-constexpr float kPromptJoin = 4.0f;
+constexpr float kPromptJoin = 4.0f, kPromptLeast = 0.28f;
 
 // The sequences of one lane each, from b0 on; by a warp.
 struct PromptSeqs {
@@ -187,12 +186,13 @@ __device__ __forceinline__ float warp_sum(float x) {
 //               items or long ones of one length (the next chunk of a prompt), which would leave CTAs idle.  An item counts as
 //               many units as the last of its sequence has key tiles, and kPromptItem more for its beginning and end.  What CTAs
 //               have of an item that they share goes through the workspace to a second kernel, which takes as long as
-//               kPromptJoin key tiles.
+//               kPromptJoin key tiles, and longer the more parts an item has: shares are no smaller than kPromptLeast
+//               times the square root of the longest item, and CTAs without one stay idle.
 // Which of the two ends sooner is estimated: whole items end with the longest, or half of the shortest of a sequence (on
 // average over the work) behind an even share.
 struct PromptShare {
-    int each, more;
-    __device__ __forceinline__ int begin(int x) const { return each * x + min(x, more); }
+    int each, more, all;
+    __device__ __forceinline__ int begin(int x) const { return min(each * x + min(x, more), all); }
     __device__ __forceinline__ int owner(int u) const { return u < (each + 1) * more ? u / (each + 1) : more + (u - (each + 1) * more) / each; }
 };
 // `first`: the sequences from 0 on
@@ -214,7 +214,8 @@ __device__ __forceinline__ PromptShare prompt_share(const PromptParams &p, const
     items = warp_sum(items), tiles = warp_sum(tiles), units = warp_sum(units), least = warp_sum(least);
     const float ctas = static_cast<float>(p.ctas), most = static_cast<float>(__reduce_max_sync(0xffffffffu, longest));
     const float whole = items <= ctas ? most : fmaxf(most, tiles / ctas + 0.5f * least / fmaxf(tiles, 1.0f));
-    if (units > 1e9f || whole <= units / ctas + kPromptJoin) return {0, 0};
+    const float least_share = kPromptLeast * sqrtf(most + kPromptItem);
+    if (units > 1e9f || whole <= fmaxf(units / ctas, least_share) + kPromptJoin) return {0, 0, 0};
     int all = 0;
     q = first;
     for (int b0 = 0;;) {
@@ -224,8 +225,9 @@ __device__ __forceinline__ PromptShare prompt_share(const PromptParams &p, const
         q = PromptSeqs(p, b0);
     }
     all = __reduce_add_sync(0xffffffffu, all);
-    const int each = all / p.ctas;
-    return {each, all - each * p.ctas};  // (each > 0: whole items are as good where there are fewer units than CTAs)
+    const int each = all / p.ctas, wanted = static_cast<int>(least_share) + 1;
+    if (each < wanted) return {wanted, 0, all};
+    return {each, all - each * p.ctas, all};
 }
 
 // 32 sequences in the order of the work: those with the longest contexts first, so that what begins late is short.  A lane's sequence
@@ -334,32 +336,6 @@ __device__ __forceinline__ uint4 transposed4(const uint32_t (&w)[4]) {
     return upper ? make_uint4(s0, s1, a2, a3) : make_uint4(a0, a1, s0, s1);
 }
 
-// 2^y on the multiply-add units, for both halves of y (Cody and Waite's reduction: y = n + f with n whole and |f| <= 1/2; a
-// polynomial for 2^f, of the least largest relative error; n into the exponent).  y is at most 64 or so, and what is
-// below -126 counts as -126.  The polynomial is off by 2.6e-6, less than a hundredth of half a step of fp16, or 7.5e-5, a
-// fiftieth of half a step of bf16.
-template <class T>
-__device__ __forceinline__ float2 exp2_poly(float2 y) {
-    const auto both = [](float x) { return pair32(x, x); };
-    const uint64_t yy = pair32(fmaxf(y.x, -126.0f), fmaxf(y.y, -126.0f));
-    const uint64_t t = add2(yy, both(12582912.0f));  // 1.5 * 2^23: the whole part ends in the low bits
-    const uint64_t f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), yy);
-    uint64_t r;
-    if constexpr (F16Kind<T>::kType == 0) {
-        r = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
-        r = fma2(r, f, both(0.240247443318367f));
-        r = fma2(r, f, both(0.6931217908859253f));
-        r = fma2(r, f, both(0.9999992847442627f));
-    } else {
-        r = fma2(both(0.0551716685295105f), f, both(0.2426111251115799f));
-        r = fma2(r, f, both(0.6932609677314758f));
-        r = fma2(r, f, both(0.9999280571937561f));
-    }
-    const float2 v = unpair32(r), n = unpair32(t);
-    return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(n.x) << 23)),
-                       __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(n.y) << 23)));
-}
-
 // A thread's row of one tile of scores becomes a row of weights, in tensor memory.  m: the maximum that the weights are taken against,
 // l: their sum so far.
 template <class T, int D>
@@ -426,13 +402,8 @@ struct SoftmaxRow {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 float2 y = unpair32(fma2(pair32(score(16 * q + 2 * x), score(16 * q + 2 * x + 1)), c2, mc2));
-                // some on the multiply-add units, which have time to spare (where nothing is hidden: 2^-infinity is 0)
-                if (!kAny && x % 8 >= 8 - kPromptPoly) {
-                    y = exp2_poly<T>(y);
-                } else {
-                    y.x = exp2_fast(y.x);
-                    y.y = exp2_fast(y.y);
-                }
+                y.x = exp2_fast(y.x);
+                y.y = exp2_fast(y.y);
                 sums[x % 4] = add2(sums[x % 4], pair32(y.x, y.y));
                 w[x] = pack16<T>(y.x, y.y);
             }
@@ -547,6 +518,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (!shared || index < 0 || index >= p.ctas) return;
                 unit = share.begin(index);
                 unit_end = share.begin(index + 1);
+                if (unit == unit_end && lane == 0) prompt_crossings(p)[index] = crossing;  // (nothing)
             };
             const auto ask = [&]() {
                 if (lane == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
@@ -855,6 +827,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll 1
                 for (int q = 0; q < D / 16; ++q) {
                     uint32_t u[16] = {};
+                    __syncwarp();  // (rows differ in what they add)
                     if (tiles > 0) {
                         tmem_ld16(o_at + 16 * q, u);
                         tmem_wait_ld(u);
@@ -931,41 +904,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
 }
 
-// Joins what several CTAs have of an item.  Block x has the item that begins in CTA x.
+// Joins what several CTAs have of an item, in the order of the keys.  Blocks (., x) have the item that begins in CTA x, 32 rows each, so
+// that one with many parts is read by several SMs; eight lanes have a row.
+constexpr int kJoinRows = 32;
 template <class T, int D>
-__global__ void __launch_bounds__(1024) prompt_join_kernel(const PromptParams p) {
+__global__ void __launch_bounds__(8 * kJoinRows) prompt_join_kernel(const PromptParams p) {
     grid_dep_wait();
     if (reinterpret_cast<const PromptHead *>(p.workspace)->shared == 0) return;
-    const PromptItem it = prompt_crossings(p)[blockIdx.x];
+    const PromptItem it = prompt_crossings(p)[blockIdx.y];
     if (it.ctas == 0) return;
-    const auto slot = [&](int s) { return prompt_slot(p, D, s == 0 ? it.slot : 2 * (static_cast<int>(blockIdx.x) + s)); };
+    const auto slot = [&](int s) { return prompt_slot(p, D, s == 0 ? it.slot : 2 * (static_cast<int>(blockIdx.y) + s)); };
     constexpr int kPieces = D / 32;  // of four columns, 32 columns apart
-    // eight lanes have a row
-    for (int row = threadIdx.x / 8; row < 256; row += 128) {
-        const int lane = threadIdx.x % 8, tok = row % 128 / p.group, token = it.token0 + row / 128 * p.tile_tokens + tok;
-        if (tok >= p.tile_tokens || token >= it.n) continue;
-        float top = -INFINITY, sum = 0.0f, acc[kPieces][4] = {};
-#pragma unroll 2
-        for (int s = 0; s < it.ctas; ++s) {
-            const float2 ml = *reinterpret_cast<const float2 *>(slot(s) + 256 * D + 2 * row);
-            if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part whose keys the row does not see: it has no sums
-            float f[kPieces][4];
+    const int row = static_cast<int>(blockIdx.x) * kJoinRows + static_cast<int>(threadIdx.x) / 8;
+    const int lane = threadIdx.x % 8, tok = row % 128 / p.group, token = it.token0 + row / 128 * p.tile_tokens + tok;
+    if (tok >= p.tile_tokens || token >= it.n) return;
+    float top = -INFINITY, sum = 0.0f, acc[kPieces][4] = {};
+#pragma unroll 4
+    for (int s = 0; s < it.ctas; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(slot(s) + 256 * D + 2 * row);
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part whose keys the row does not see: it has no sums
+        float f[kPieces][4];
 #pragma unroll
-            for (int q = 0; q < kPieces; ++q) load_floats(slot(s) + row * D + 32 * q + 4 * lane, f[q]);
-            const float to = fmaxf(top, ml.x), old = top == -INFINITY ? 0.0f : exp2_fast(top - to), w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - to);
-            top = to;
-            sum = sum * old + w * ml.y;
-#pragma unroll
-            for (int q = 0; q < kPieces; ++q)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) acc[q][x] = acc[q][x] * old + w * f[q][x];
-        }
-        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-        T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + row % 128 - tok * p.group) * D + 4 * lane;
+        for (int q = 0; q < kPieces; ++q) load_floats(slot(s) + row * D + 32 * q + 4 * lane, f[q]);
+        const float to = fmaxf(top, ml.x), old = top == -INFINITY ? 0.0f : exp2_fast(top - to), w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - to);
+        top = to;
+        sum = sum * old + w * ml.y;
 #pragma unroll
         for (int q = 0; q < kPieces; ++q)
-            *reinterpret_cast<uint2 *>(out + 32 * q) = make_uint2(pack16<T>(acc[q][0] * inv, acc[q][1] * inv), pack16<T>(acc[q][2] * inv, acc[q][3] * inv));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[q][x] = acc[q][x] * old + w * f[q][x];
     }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    T *out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + token) * p.out_ld + static_cast<long long>(it.head * p.group + row % 128 - tok * p.group) * D + 4 * lane;
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+        *reinterpret_cast<uint2 *>(out + 32 * q) = make_uint2(pack16<T>(acc[q][0] * inv, acc[q][1] * inv), pack16<T>(acc[q][2] * inv, acc[q][3] * inv));
 }
 
 // Tensor maps of the queries (rows of heads) and of keys or values (pages), 128-byte swizzle, boxes 64 values wide.
@@ -1022,8 +995,8 @@ inline int launch_prompt_typed(PromptParams &p, int type, bool pdl, cudaStream_t
     cfg.numAttrs = pdl ? 1 : 0;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
     if (err != cudaSuccess) return err;
-    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
-    cfg.blockDim = dim3(1024);
+    cfg.gridDim = dim3(256 / kJoinRows, static_cast<unsigned>(p.ctas));
+    cfg.blockDim = dim3(8 * kJoinRows);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, prompt_join_kernel<T, D>, p);

@@ -527,3 +527,58 @@ def test_no_tokens_is_no_work():
     q = torch.zeros((0, 4, 64), dtype=FP16, device="cuda")
     assert dmm.prompt_attention(q, k, v, table, lens, cu_of([0, 0])).shape == (0, 4, 64)
     assert dmm.append_kv(torch.zeros((0, 512), device="cuda"), k, v, table, lens, cu_seqlens=cu_of([0, 0])).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("new,past,H,Hkv,D,page,dtype", [
+    (5, 3000, 8, 1, 128, 64, FP16),
+    (1, 2000, 16, 1, 64, 16, BF16),
+    (260, 15000, 1, 1, 64, 128, FP16),   # two pairs of tiles
+    (16, 15000, 64, 1, 128, 16, BF16),
+    (3, 700, 8, 1, 128, 32, FP16),       # short enough for one CTA
+])
+def test_prompt_with_fewer_key_tiles_than_ctas(new, past, H, Hkv, D, page, dtype):
+    gen = generator(22)
+    k, v, table, lens = make_cache(gen, [new + past], Hkv, D, page, dtype)
+    q = torch.randn((new, H, D), generator=gen, device="cuda").to(dtype)
+    want, bound = attention(q, k, v, table, lens, cu_of([new]))
+    for _ in range(2):
+        got = dmm.prompt_attention(q, k, v, table, lens, cu_of([new]))
+        assert check_attention(got, want, bound) == got.numel()
+
+
+def test_captured_prompts_of_other_lengths():
+    """One captured call, replayed for lengths whose work is shared out in either way, beside another captured call on the same workspace."""
+    gen = generator(23)
+    H, Hkv, D, page = 8, 1, 128, 16
+    k, v, table, lens = make_cache(gen, [9000, 700, 5000], Hkv, D, page, FP16)
+    full = lens.clone()
+    ws = torch.empty(dmm.attention_workspace_bytes(300, 3, H, Hkv, D), dtype=torch.uint8, device="cuda")
+    q = torch.randn((300, H, D), generator=gen, device="cuda").to(FP16)
+    cu = cu_of([100, 100, 100])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        dmm.prompt_attention(q, k, v, table, lens, cu, workspace=ws, pdl=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            first = dmm.prompt_attention(q, k, v, table, lens, cu, workspace=ws, pdl=True)
+            out = dmm.prompt_attention(first, k, v, table, lens, cu, workspace=ws, pdl=True)
+        graphs.append((graph, first, out))
+    for at, new in (([9000, 700, 5000], [100, 100, 100]), ([100, 100, 100], [100, 100, 100]), ([300, 0, 17], [280, 0, 17]),
+                    ([9000, 0, 0], [3, 0, 0]), ([200, 700, 5000], [1, 298, 1])):
+        lens.copy_(torch.tensor(at))
+        cu.copy_(cu_of(new))
+        q.copy_(torch.randn(q.shape, generator=gen, device="cuda"))
+        for graph, first, out in graphs:
+            for t in (first, out):
+                t.fill_(0)
+            graph.replay()
+            rows = sum(new)
+            for x, y in ((q, first), (first, out)):
+                want, bound = attention(x, k, v, table, lens, cu)
+                assert check_attention(y, want, bound) == rows * H * D
+    assert dmm.status() == 0
+    lens.copy_(full)
