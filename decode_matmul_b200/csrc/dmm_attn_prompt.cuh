@@ -341,13 +341,13 @@ __device__ __forceinline__ uint4 transposed4(const uint32_t (&w)[4]) {
 template <class T, int D>
 struct SoftmaxRow {
     uint32_t s_at, o_at;   // tensor memory of S (then P) and O
-    float c, turn;         // weights are 2^(c turn S - c m)
+    float c;               // weights are 2^(c S - c m)
     uint32_t bar;          // barriers of the two parts of P
     int sees;              // keys of the tile that the row sees
     bool begun;            // O has a sum already
 
-    // kAny: some row does not see all keys, or the scale is not positive
-    template <bool kAny>
+    // kMasked: some row does not see all keys
+    template <bool kMasked>
     __device__ __forceinline__ void step(float &m, float &l) const {
         uint32_t u[128];
         tmem_ld32(s_at, u);
@@ -364,9 +364,9 @@ struct SoftmaxRow {
                 tmem_wait_ld32(u + 64);
                 tmem_wait_ld32(u + 96);
             }
-            if constexpr (kAny) {
+            if constexpr (kMasked) {
 #pragma unroll
-                for (int x = 64 * half; x < 64 * half + 64; ++x) u[x] = __float_as_uint(x < sees ? score(x) * turn : -INFINITY);
+                for (int x = 64 * half; x < 64 * half + 64; ++x) u[x] = x < sees ? u[x] : 0xff800000u;
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
@@ -618,8 +618,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         } else if (warp == 8) {
             // =============================== MMA ===============================
             const bool leader = elect_one();
-            // D fp32 (1 at bit 4), the operands' type, N >> 3 at bit 17, M >> 4 at bit 24; V is the operand whose rows run along N (bit 16)
-            constexpr uint32_t kIdS = (1u << 4) | F16Kind<T>::kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            // D fp32 (1 at bit 4), the operands' type, N >> 3 at bit 17, M >> 4 at bit 24; V is the operand whose rows run along N (bit 16);
+            // -Q for a scale below 0 (bit 13)
+            const uint32_t id_s = (p.scale < 0.0f ? 1u << 13 : 0u) | (1u << 4) | F16Kind<T>::kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             constexpr uint32_t kIdO = (1u << 4) | F16Kind<T>::kType | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
             // 128-byte swizzle (2 at bit 61), 8-row groups 1024 bytes apart, version 1 at bit 46; the low word has the address and, for
             // V, the distance from one 64 columns to the next
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const uint32_t off = (k / 4) * (Plan::kHalfBytes >> 4) + (k % 4) * 2;
-                        mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, kIdS, k > 0);
+                        mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, id_s, k > 0);
                     }
                     tc_commit(bar(Plan::kBarS + i));
                 }
@@ -787,9 +788,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int i = warp / 4, r = threadIdx.x % 128, magic = 65536 / p.group + 1, tok = r * magic >> 16;  // (r / group, for r < 128)
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
         const uint32_t s_at = lanes + Plan::kS + 128 * i, o_at = lanes + Plan::kO + D * i;
-        // c S <= 0 for c <= 0: such scales turn the sign of S, or make it 0
-        const float turn = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
-        const float c = turn == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
+        // (the products have the sign of the scale; times 2^-149 every finite score is as good as 0, and a hidden one stays -infinity)
+        const float c = p.scale == 0.0f ? __uint_as_float(1u) : fabsf(p.scale) * 1.4426950408889634f;
         uint32_t s_full = 0, o_full = 0;  // phases
         for (int k = 0;; ++k) {
             const PromptItem it = item_of(k);
@@ -805,8 +805,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
                 s_full ^= 1u;
                 tc_fence_after();
-                const SoftmaxRow<T, D> row = {s_at, o_at, c, turn, bar(Plan::kBarP + 2 * i), sees - (it.first + j) * kPromptKeys, j > 0};
-                if (j < free && turn == 1.0f)
+                const SoftmaxRow<T, D> row = {s_at, o_at, c, bar(Plan::kBarP + 2 * i), sees - (it.first + j) * kPromptKeys, j > 0};
+                if (j < free)
                     row.template step<false>(m, l);
                 else
                     row.template step<true>(m, l);

@@ -582,3 +582,18 @@ def test_captured_prompts_of_other_lengths():
                 assert check_attention(y, want, bound) == rows * H * D
     assert dmm.status() == 0
     lens.copy_(full)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_scale_of_zero_means_the_average(dtype):
+    # also where a score would be infinite in the type of the queries
+    gen = generator(24)
+    k, v, table, lens = make_cache(gen, [300, 20], 2, 128, 16, dtype)
+    big = 60000.0 if dtype == FP16 else 1e15
+    q = (big * torch.randn((320, 4, 128), generator=gen, device="cuda").clamp(-1, 1)).to(dtype)
+    want, bound = attention(q, k, v, table, lens, cu_of([300, 20]), 0.0)
+    got = dmm.prompt_attention(q, k, v, table, lens, cu_of([300, 20]), 0.0)
+    assert check_attention(got, want, bound) == got.numel()
+    rows = torch.tensor([299, 319], device="cuda")
+    one = dmm.paged_attention(q[rows], k, v, table, lens, 0.0)
+    assert check_attention(one, want[rows], bound[rows]) == one.numel()
