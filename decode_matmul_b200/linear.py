@@ -122,6 +122,8 @@ class LinearStack:
         # faster on B200 (77.5 against 91 us per block): the hardware's dependent-launch hand-over
         # beats a software barrier between resident CTAs
         self.chain_blocks = 0
+        self._kept = {}         # buffers whose addresses a captured step has, by batch
+        self._captured = []     # buffers that were made while a step was captured
 
     def step(self, h: torch.Tensor, path: int = _lib.PATH_AUTO, fused: bool | None = None, cache=None,
              cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
@@ -129,7 +131,7 @@ class LinearStack:
 
         ``cache`` (a :class:`PagedCache` of this rank's key heads, fp16): the blocks attend.  The rows of ``h`` are the new
         tokens of its sequences, for which :meth:`PagedCache.extend` has made room; ``cu_seqlens`` is what that returned, None
-        for one token per sequence.
+        for one token per sequence.  Rows behind the last sequence pass the blocks without attention.
 
         ``fused`` (default: whenever the batch is at most 32): every elementwise step between two
         layers runs inside the matmul kernels -- the loaders read fp32 and round to fp16 or form
@@ -159,7 +161,10 @@ class LinearStack:
 
         view = (cache.k(i), cache.v(i), cache.page_table, cache.seq_lens)
         q = append_kv(a, *view, self._freqs, cu_seqlens=cu_seqlens, pdl=pdl)
-        out = paged_attention(q, *view, pdl=pdl) if cu_seqlens is None else prompt_attention(q, *view, cu_seqlens, pdl=pdl)
+        if cu_seqlens is None:
+            out = paged_attention(q, *view, pdl=pdl)
+        else:  # (rows behind the last sequence have no attention: o reads zeros)
+            out = prompt_attention(q, *view, cu_seqlens, output=torch.zeros_like(q), pdl=pdl)
         return out.view(out.shape[0], -1)
 
     def _step_attend(self, h: torch.Tensor, cache, cu_seqlens, path: int, fused: bool) -> torch.Tensor:
@@ -170,6 +175,8 @@ class LinearStack:
         if cache.layers != len(self.layers) or cache.kv_heads != kv_heads or cache.head_dim != head_dim or cache.pages.dtype != torch.float16:
             raise RuntimeError(f"cache must be fp16, of {len(self.layers)} layers with {kv_heads} key heads of {head_dim}")
         if getattr(self, "_freqs", None) is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first step with a cache cannot be captured: run one before")
             self._freqs = rotary_frequencies(head_dim, self.cfg.get("rope_base", 10000.0), device=self.device)
         ffn_loc = self.ffn // self.world
         if not fused:
@@ -195,17 +202,25 @@ class LinearStack:
 
     def _buffers(self, batch: int):
         key = (batch,)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if batch in self._kept:
+            return self._kept[batch]
         if getattr(self, "_buf_key", None) != key:
             n_qkv = self.layers[0]["qkv"].out_features
             n_gu = self.layers[0]["gate_up"].out_features
             mk = lambda n: torch.zeros((batch, n), dtype=torch.float32, device=self.device)
-            self._buf = {"a": mk(n_qkv), "g": mk(n_gu), "po": mk(self.hidden), "pd": mk(self.hidden)}
+            buf = {"a": mk(n_qkv), "g": mk(n_gu), "po": mk(self.hidden), "pd": mk(self.hidden)}
             # scratch of this stack's own (two stacks on two streams must not share the library's buffer)
             from .ops import workspace_bytes
 
             need = max(workspace_bytes(batch, lin.out_features, lin.in_features) for lin in self.layers[0].values())
-            self._buf["ws"] = torch.zeros((need,), dtype=torch.uint8, device=self.device)
-            self._buf_key = key
+            buf["ws"] = torch.zeros((need,), dtype=torch.uint8, device=self.device)
+            if capturing:  # (filled when the graph runs: the graph's alone)
+                self._captured.append(buf)
+                return buf
+            self._buf, self._buf_key = buf, key
+        if capturing:  # a step on another batch must not free what the graph goes on using
+            self._kept[batch] = self._buf
         return self._buf
 
     def _peer_state(self, batch: int):

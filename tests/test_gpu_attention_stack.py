@@ -145,3 +145,62 @@ def test_without_a_cache_nothing_has_changed():
         g = blk["gate_up"](b.to(torch.float16))
         blk["down"]((torch.nn.functional.silu(g[:, :CFG["ffn"]]) * g[:, CFG["ffn"]:]).to(torch.float16), out=b, accumulate=True)
     assert torch.equal(a, b)
+
+
+def test_a_captured_step_outlives_steps_of_other_batches():
+    """Prompts that come between the replays of a captured step take other buffers than the graph's, and leave those alone."""
+    stack, cache, twin = stack_of(CFG), cache_of(CFG), cache_of(CFG)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    start = torch.randn((3 * 20, CFG["hidden"]), generator=gen, device="cuda")
+    for c in (cache, twin):
+        stack.step(start.clone(), cache=c, cu_seqlens=c.extend([20, 20, 20]))
+    h = torch.zeros((3, CFG["hidden"]), device="cuda")
+    cache.extend([1, 1, 1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        stack.step(h, cache=cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stack.step(h, cache=cache)
+    kept = [t.data_ptr() for t in stack._buffers(3).values()]
+    cache.seq_lens -= 1
+    cache.lengths = [n - 1 for n in cache.lengths]
+    for i in range(6):
+        x = torch.randn((3, CFG["hidden"]), generator=gen, device="cuda")
+        assert cache.extend([1, 1, 1]) is None and twin.extend([1, 1, 1]) is None
+        h.copy_(x)
+        graph.replay()
+        near(h, stack.step(x.clone(), cache=twin), CFG["layers"])
+        rows = torch.randn((5 + i, CFG["hidden"]), generator=gen, device="cuda")
+        for c in (cache, twin):
+            stack.step(rows.clone(), cache=c, cu_seqlens=c.extend([i, 5, 0]))
+        assert [t.data_ptr() for t in stack._buffers(3).values()] == kept
+        assert not {t.data_ptr() for t in stack._buffers(5 + i).values()} & set(kept)
+    assert dmm.status() == 0
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_rows_behind_the_last_sequence(fused):
+    """A padded batch: its last rows are no sequence's; the others are as without them, the cache too."""
+    stack, cache, twin = stack_of(CFG), cache_of(CFG), cache_of(CFG)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    rows = torch.randn((13, CFG["hidden"]), generator=gen, device="cuda")
+    del [torch.full((21, CFG["hidden"]), math.nan, dtype=torch.float16, device="cuda") for _ in range(16)][:]  # (what new tensors may lie on)
+    got = stack.step(torch.cat([rows, rows[:8]]), cache=cache, cu_seqlens=cache.extend([4, 0, 9]), fused=fused)
+    want = stack.step(rows.clone(), cache=twin, cu_seqlens=twin.extend([4, 0, 9]), fused=fused)
+    near(got[:13], want, CFG["layers"])
+    assert bool(torch.isfinite(got).all()) and dmm.status() == 0
+    near(cache.pages.float(), twin.pages.float(), CFG["layers"])
+
+
+def test_the_first_step_with_a_cache_is_not_captured():
+    stack, cache = stack_of(CFG), cache_of(CFG)
+    h = torch.zeros((3, CFG["hidden"]), device="cuda")
+    cache.extend([1, 1, 1])
+    stack.step(h, fused=False)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            stack.step(h, cache=cache)
