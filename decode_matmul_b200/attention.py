@@ -99,6 +99,17 @@ def _check_rows(t, name, dtype, index, head_dim):
     return tokens, heads, ld if tokens > 1 else heads * head_dim
 
 
+def _overlap(a, a_ld, a_width, b, b_ld, b_width, rows):
+    """Whether rows of a and b (widths and distances in bytes) share memory: rows of one buffer side by side do not."""
+    a_at, b_at = a.data_ptr(), b.data_ptr()
+    if a_at + (rows - 1) * a_ld + a_width <= b_at or b_at + (rows - 1) * b_ld + b_width <= a_at:
+        return False
+    if a_ld != b_ld or rows == 1:
+        return True
+    apart = (b_at - a_at) % a_ld
+    return apart < a_width or apart + b_width > a_ld
+
+
 def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=None, *, cu_seqlens=None, interleaved=False, pdl=False):
     """Rotated queries [tokens, heads, head_dim] of the cache's type, and new rows of the cache, from the result of a qkv
     product.
@@ -107,7 +118,8 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
     ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32 [sequences + 1]) are the last tokens of sequence b, whose
     ``seq_lens[b]`` counts them; without ``cu_seqlens`` there is one token per sequence.  Queries and keys are rotated by
     their position times ``freqs`` (float64 [head_dim / 2], :func:`rotary_frequencies`; None: not rotated), the two
-    halves of a head as pairs or, ``interleaved``, neighbours.  Rows behind the last sequence are skipped."""
+    halves of a head as pairs or, ``interleaved``, neighbours.  Rows behind the last sequence are skipped.  No two tokens
+    of a call may have the same place in the cache; ``output`` may be the query heads of a 16-bit ``qkv`` themselves."""
     cache, dtype, index, kv_heads, head_dim, seqs = _check_cache(k_pages, v_pages, page_table, seq_lens)
     kind = _TYPE_IN.get(qkv.dtype) if isinstance(qkv, torch.Tensor) else None
     if kind is None:
@@ -136,6 +148,10 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
         rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
         if rows != tokens or out_heads != heads:
             _no("output must be [tokens, heads, head_dim]")
+        size = qkv.element_size()
+        if tokens > 0 and _overlap(qkv, size * (qkv.stride(0) if tokens > 1 else width), size * width, output, 2 * out_ld, 2 * heads * head_dim, tokens) and (
+                output.data_ptr() != qkv.data_ptr() or qkv.dtype is not dtype or (tokens > 1 and out_ld != qkv.stride(0))):
+            _no("output must be the query heads of qkv or share no memory with it")
     if tokens == 0:
         return output
     args = (qkv.data_ptr(), kind, qkv.stride(0) if tokens > 1 else width, tokens, heads, None if freqs is None else freqs.data_ptr(),
@@ -174,8 +190,8 @@ def _attend(name, q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, scale, 
         rows, out_heads, out_ld = _check_rows(output, "output", dtype, index, head_dim)
         if rows != tokens or out_heads != heads:
             _no("output must have the shape of q")
-        if tokens > 0 and output.data_ptr() == q.data_ptr():
-            _no("output must not be q")
+        if tokens > 0 and _overlap(q, 2 * q_ld, 2 * heads * head_dim, output, 2 * out_ld, 2 * heads * head_dim, tokens):
+            _no("output must not be q or share memory with it")
     if tokens == 0:
         return output
     if scale is None:
@@ -212,7 +228,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, scale=None, outpu
     """Attention of one new token per sequence: [sequences, heads, head_dim] of the cache's type.
 
     ``q`` is [sequences, heads, head_dim]; query head h reads key head h // (heads / kv_heads), over the ``seq_lens[b]``
-    keys of its sequence.  ``scale`` defaults to head_dim ** -0.5.  A sequence of length 0 gets zeros.  ``workspace``: scratch
+    keys of its sequence.  ``scale`` defaults to head_dim ** -0.5.  A sequence of length 0 gets zeros.  Sequences may share pages.
+    ``workspace``: scratch
     of at least :func:`attention_workspace_bytes` bytes, not shared with calls that may overlap on the GPU; by default the
     call allocates its own."""
     return _attend("paged_attention", q, k_pages, v_pages, page_table, seq_lens, None, scale, output, workspace, pdl)

@@ -189,6 +189,9 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Of a sum of weights: 0 where there is none (no keys, or scores that are all -infinity), so that the result is 0.
+__device__ __forceinline__ float decode_inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+
 // What a warp has of one segment when it could not write it out.
 struct DecodePart {
     long long start;
@@ -398,7 +401,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                     if (have == at.units) {
                         const int r = at.tile * Plan::kRows + 8 * t + quad;
                         T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head) * p.group + r) * D + 2 * pair;
-                        const float i0 = at.len > 0 ? 1.0f / l[t][0] : 0.0f, i1 = at.len > 0 ? 1.0f / l[t][1] : 0.0f;
+                        const float i0 = decode_inverse(l[t][0]), i1 = decode_inverse(l[t][1]);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             }
             if (whole) {
                 T *out = static_cast<T *>(p.out) + of.seq * p.out_ld + (static_cast<long long>(of.head) * p.group + of.tile * Plan::kRows + row) * D + kC * lane;
-                const float inv = 1.0f / sum;
+                const float inv = decode_inverse(sum);
 #pragma unroll
                 for (int y = 0; y < kC; y += 2) *reinterpret_cast<uint32_t *>(out + y) = pack16<T>(acc[y] * inv, acc[y + 1] * inv);
             } else {
@@ -567,8 +570,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_join_kernel(const Dec
             a += f * s_acc[w][2 * threadIdx.x];
             b += f * s_acc[w][2 * threadIdx.x + 1];
         }
+        const float inv = decode_inverse(sum);
         T *out = static_cast<T *>(p.out) + at.seq * p.out_ld + (static_cast<long long>(at.head) * p.group + r) * D;
-        *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack16<T>(a / sum, b / sum);
+        *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack16<T>(a * inv, b * inv);
     }
 }
 

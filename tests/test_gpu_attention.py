@@ -597,3 +597,57 @@ def test_scale_of_zero_means_the_average(dtype):
     rows = torch.tensor([299, 319], device="cuda")
     one = dmm.paged_attention(q[rows], k, v, table, lens, 0.0)
     assert check_attention(one, want[rows], bound[rows]) == one.numel()
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_in_place(dtype, interleaved):
+    gen = generator(25)
+    new, past = [70, 1, 0, 9], [5, 0, 3, 500]
+    total = [n + p for n, p in zip(new, past)]
+    k, v, table, lens = make_cache(gen, total, 2, 64, 16, dtype)
+    k2, v2 = k.clone(), v.clone()
+    qkv = torch.randn((sum(new), 9 * 64), generator=gen, device="cuda").to(dtype)
+    freqs, cu = dmm.rotary_frequencies(64, device="cuda"), cu_of(new)
+    want = dmm.append_kv(qkv, k, v, table, lens, freqs, cu_seqlens=cu, interleaved=interleaved)
+    same = qkv.clone()
+    heads = same.view(-1, 9, 64)[:, :5]
+    assert dmm.append_kv(same, k2, v2, table, lens, freqs, heads, cu_seqlens=cu, interleaved=interleaved) is heads
+    assert torch.equal(heads, want) and torch.equal(same[:, 5 * 64:], qkv[:, 5 * 64:])
+    assert torch.equal(torch.nan_to_num(k), torch.nan_to_num(k2)) and torch.equal(torch.nan_to_num(v), torch.nan_to_num(v2))
+
+
+def test_outputs_in_the_way_of_inputs_are_refused():
+    gen = generator(26)
+    k, v, table, lens = make_cache(gen, [20, 30], 2, 64, 16, FP16)
+    wide = torch.randn((2, 12, 64), generator=gen, device="cuda").to(FP16)
+    q, cu = wide[:, :4], cu_of([1, 1])
+    want = dmm.paged_attention(q.contiguous(), k, v, table, lens)
+    for call in (lambda out: dmm.paged_attention(q, k, v, table, lens, None, out), lambda out: dmm.prompt_attention(q, k, v, table, lens, cu, None, out)):
+        for at in (0, 1, 3):
+            with pytest.raises(RuntimeError, match="share memory"):
+                call(wide[:, at:at + 4])
+        with pytest.raises(RuntimeError, match="share memory"):
+            call(torch.as_strided(wide, (2, 4, 64), (13 * 64, 64, 1), 64))
+    assert torch.equal(dmm.paged_attention(q, k, v, table, lens, None, wide[:, 4:8]), want)  # side by side in one buffer
+    qkv = wide[:, :8].flatten(1)
+    for at in (1, 4):
+        with pytest.raises(RuntimeError, match="share no memory"):
+            dmm.append_kv(qkv, k, v, table, lens, None, qkv.view(2, 8, 64)[:, at:at + 4])
+    big = torch.zeros((2, 8 * 64), device="cuda")
+    with pytest.raises(RuntimeError, match="share no memory"):
+        dmm.append_kv(big, k, v, table, lens, None, big.view(FP16).view(2, 16, 64)[:, :4])
+
+
+def test_scores_that_are_all_minus_infinity_give_zeros():
+    # a weight of 0 for every key: as without keys.  Short and long, so that parts are joined as well
+    gen = generator(27)
+    k, v, table, lens = make_cache(gen, [40, 9000, 17], 1, 128, 64, BF16)
+    for b, n in enumerate((40, 9000)):
+        pos = torch.arange(n, device="cuda")
+        k[table[b].long()[pos // 64], :, pos % 64] = -math.inf
+    q = torch.rand((3, 4, 128), generator=gen, device="cuda").to(BF16) + 0.5
+    want, bound = attention(q, k, v, table, lens, None)
+    for got in (dmm.paged_attention(q, k, v, table, lens), dmm.prompt_attention(q, k, v, table, lens, cu_of([1, 1, 1]))):
+        assert bool((got[:2] == 0).all())
+        assert check_attention(got[2], want[2], bound[2]) == 4 * 128
