@@ -6,7 +6,11 @@
 //
 // A block has one token and some of its heads.  The D / 2 sines and cosines of the token are worked out once per block
 // into shared memory; then a thread takes 16 values of a head at a time, as two runs of 8 (the two halves of 8 pairs, or 8
-// neighbouring pairs), so that every load and store is 16 bytes wide.
+// neighbouring pairs), so that every load and store is 16 bytes wide, and asks for its next 16 before it works on these.
+//
+// Bound: bytes, 4 (fp32) or 2 read and 2 written for each value.  B200, graph: 2048 tokens of 64 + 16 heads of 128, fp32 in,
+// 22.0 us (5.7 TB/s, 88 % of what a copy reaches); 8164 tokens of prompts of many lengths 81 us (6.2 TB/s, 94 %).  One token
+// takes 2.1 us, a launch and three dependent loads: its sequence's length and page and the row itself.
 #pragma once
 
 #include "dmm_attn_common.cuh"
@@ -126,7 +130,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
 template <class TIn, class T, int D>
 inline int launch_append_typed(const AppendParams &p, int num_sms, bool pdl, cudaStream_t stream) {
     const int units = (p.heads + 2 * p.cache.kv_heads) * (D / 16);
-    // few tokens: a thread takes one unit, so that all of the GPU loads at once
+    // Few tokens: a thread takes one unit, so that all of the GPU loads at once (one token of 80 heads 2.1 us against 3.6 with one
+    // block for the token, 32 tokens of 96 heads 2.6 against 4.3); many: a block keeps its token, whose sines and cosines it works out
+    // once (8164 tokens 81 us against 92).
     int parts = (units + kAppendThreads - 1) / kAppendThreads;
     if (static_cast<long long>(parts) * p.tokens > 16ll * num_sms) parts = 1;
     cudaLaunchConfig_t cfg = {};

@@ -352,7 +352,7 @@ int dmm_set_wait_limit_ms(unsigned ms);
  *   k + page_table[b * table_stride + pos / page_size] * page_stride + h * head_stride + (pos % page_size) * row_stride
  * head_dim contiguous values of `type`; the strides are in elements, the same for k and v, multiples of 8, in any order of
  * the three dimensions that lets no two rows overlap.  page_size is a power of two, 16 or more; head_dim is 64 or 128;
- * k and v are 16-byte aligned.
+ * k and v are 16-byte aligned; a row of the table holds up to 2^30 tokens (max_pages * page_size).
  * seq_lens[b] is the length of sequence b in tokens, those of the present call included; table entries behind a
  * sequence's last page are not read.
  * page_table, seq_lens and cu_seqlens are device memory, so a captured graph serves sequences as they grow.  No kernel
@@ -379,7 +379,9 @@ typedef struct dmm_paged_cache {
  * (2 i, 2 i + 1) with `interleaved`.  freqs NULL: no rotation.  The angle is reduced in 64 bits, the rotation is done in 32
  * and rounded once to the cache's type.  q_out: [tokens, heads * head_dim] of the cache's type, rows q_ld apart.
  * Rows of qkv behind the last sequence and tokens at negative positions (more new tokens than the length says, which
- * raises DMM_STATUS_BAD_PAGE) are skipped: neither q_out nor the cache is written for them.  flags: DMM_FLAG_PDL only.
+ * raises DMM_STATUS_BAD_PAGE) are skipped: neither q_out nor the cache is written for them.  No two tokens of a call may have
+ * the same place in the cache.  q_out may be the query heads of a 16-bit qkv themselves (q_out == qkv, q_ld == qkv_ld), else it
+ * shares no memory with qkv.  flags: DMM_FLAG_PDL only.
  */
 int dmm_append_kv(const void *qkv, int qkv_type, int64_t qkv_ld, int64_t tokens, int heads, const double *freqs,
                   int interleaved, void *q_out, int64_t q_ld, const dmm_paged_cache *cache, const int32_t *cu_seqlens,
@@ -389,7 +391,8 @@ int dmm_append_kv(const void *qkv, int qkv_type, int64_t qkv_ld, int64_t tokens,
  * Attention of one new token per sequence: out[b, h] = sum_j softmax_j(scale * q[b, h] . k[j, h / group]) v[j, h / group]
  * over the keys j < seq_lens[b], group = heads / kv_heads (at most 128).  q and out: [num_seqs, heads, head_dim] of
  * the cache's type, q_ld / out_ld elements from one sequence to the next (multiples of 8), 16-byte aligned.  A sequence
- * of length 0 gets zeros.  The keys of all sequences are cut into equal shares, one per CTA; what shares of one sequence
+ * of length 0 gets zeros, and so does a row whose scores are all -infinity; otherwise values that are not finite show in the rows
+ * that see them, and in no others.  out shares no memory with q or the cache; sequences may share pages.  The keys of all sequences are cut into equal shares, one per CTA; what shares of one sequence
  * have in common is joined in a fixed order, so equal inputs give equal bits.  workspace: scratch of
  * dmm_attention_workspace_bytes, 256-byte aligned, of any content; calls that can overlap on the GPU need distinct ones.
  * flags: DMM_FLAG_PDL only.
