@@ -151,6 +151,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -339,14 +344,6 @@ __device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&u)[16]) 
           "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
         : "r"(taddr)
         : "memory");
-}
-// Of four lanes, lane q has words (q, 0..3) of a 4 x 4 matrix and gets (0..3, q).
-__device__ __forceinline__ uint4 transposed4(const uint32_t (&w)[4]) {
-    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
-    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? w[2] : w[3], 1);
-    const uint32_t a0 = odd ? r0 : w[0], a1 = odd ? w[1] : r0, a2 = odd ? r1 : w[2], a3 = odd ? w[3] : r1;
-    const uint32_t s0 = __shfl_xor_sync(0xffffffffu, upper ? a0 : a2, 2), s1 = __shfl_xor_sync(0xffffffffu, upper ? a1 : a3, 2);
-    return upper ? make_uint4(s0, s1, a2, a3) : make_uint4(a0, a1, s0, s1);
 }
 
 // A thread's row of one tile of scores becomes a row of weights, in tensor memory.  m: the maximum that the weights are taken against,
@@ -866,7 +863,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                 }
             } else {
-                // 8 rows of 64 bytes with each store: a row at a time would touch 32 lines
+                // 8 rows of 32 bytes with each store: a row at a time would touch 32 lines.  (Rows of 16 bytes, which need no exchange, and of 64,
+                // which need four, take 2 % longer over prompts of a few hundred tokens.)
+                const bool odd = lane & 1;
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {  // 16 rows
                     uint32_t u[D / 32][16] = {};
@@ -881,7 +880,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         const int in_warp = 16 * h + 8 * e + lane / 4, rr = 32 * (warp % 4) + in_warp, t = rr * magic >> 16;
                         const float f = __shfl_sync(0xffffffffu, inv, in_warp);
                         const bool there = t < tt && it.token0 + i * tt + t < it.n;
-                        T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + 8 * (lane % 4);
+                        T *to = out + static_cast<long long>(t) * p.out_ld + (rr - t * p.group) * D + (odd ? 8 : 0) + lane % 4 / 2 * 4;
                         if (part) {
                             if (tiles > 0 && there)
 #pragma unroll
@@ -895,10 +894,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         for (int q = 0; q < D / 32; ++q) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                w[x] = pack16<T>(__uint_as_float(u[q][4 * x + 2 * e]) * f, __uint_as_float(u[q][4 * x + 2 * e + 1]) * f);
-                            const uint4 piece = transposed4(w);
-                            if (there) *reinterpret_cast<uint4 *>(to + 32 * q) = piece;
+                            for (int x = 0; x < 4; ++x) {
+                                const float2 v = unpair32(mul2(pair32(__uint_as_float(u[q][4 * x + 2 * e]), __uint_as_float(u[q][4 * x + 2 * e + 1])), pair32(f, f)));
+                                w[x] = pack16<T>(v.x, v.y);
+                            }
+#pragma unroll
+                            for (int x = 0; x < 4; x += 2) {  // (neighbouring lanes exchange a word: 4 columns a lane, 16 of a row)
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[x] : w[x + 1], 1);
+                                if (there) *reinterpret_cast<uint2 *>(to + 32 * q + 8 * x) = make_uint2(odd ? got : w[x], odd ? w[x + 1] : got);
+                            }
                         }
                     }
                 }
