@@ -18,6 +18,7 @@ from . import _lib
 
 _TYPE_16 = {torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
 _pack = _lib.paged_cache.pack
+_scratch = {}  # bytes of scratch by device and head size, on which alone they depend
 _TYPE_IN = {torch.float32: _lib.T_F32, **_TYPE_16}
 
 
@@ -211,7 +212,9 @@ def _launch(q, q_ld, tokens, heads, scale, output, out_ld, cache, cu_seqlens, wo
     L = _lib.lib()
     if workspace is None:
         # scratch of this call's own, of 16-bit values: the caching allocator knows about streams and captured graphs
-        ws_bytes = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
+        ws_bytes = _scratch.get((index, head_dim))
+        if ws_bytes is None:
+            ws_bytes = _scratch[index, head_dim] = L.dmm_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim)
         workspace = q.new_empty(((ws_bytes + 1) // 2,))
     elif not isinstance(workspace, torch.Tensor) or workspace.get_device() != index or not workspace.is_contiguous():
         _no(f"workspace must be a contiguous tensor on device {index}")
