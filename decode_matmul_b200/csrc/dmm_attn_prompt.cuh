@@ -449,9 +449,10 @@ __device__ __forceinline__ int next_block(uint32_t answer) {
 }
 
 // What follows from an item: its key tiles for each of its two tiles (from `first` on), how many keys their last rows see, and the first
-// key tile in which a row ends (or the sequence).  Row t of the new tokens sees keys below len - n + t + 1.
+// key tile in which a row ends (or the sequence).  Row t of the new tokens sees keys below len - n + t + 1; all rows see those below
+// `seen`.
 struct PromptExtent {
-    int tiles[2], most[2], all, guarded;
+    int tiles[2], most[2], all, seen, guarded;
     __device__ __forceinline__ PromptExtent(const PromptItem &it, int tile_tokens) {
         const int shift = it.len - it.n + 1;
 #pragma unroll
@@ -461,7 +462,8 @@ struct PromptExtent {
             tiles[i] = max(0, min(it.end, (most[i] + kPromptKeys - 1) / kPromptKeys) - it.first);
         }
         all = it.end - it.first;
-        guarded = max(0, shift + it.token0) / kPromptKeys;
+        seen = max(0, shift + it.token0);
+        guarded = seen / kPromptKeys;
     }
 };
 
@@ -751,7 +753,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
                 for (int j = max(0, ext.guarded - it.first); j < ext.all; ++j) {
-                    const int rows = min(kPromptKeys, it.len - (it.first + j) * kPromptKeys), g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
+                    // rows of values behind the first that not every query sees (or all of them, where the sequence ends)
+                    const int rows = min(kPromptKeys, it.len - (it.first + j) * kPromptKeys), row0 = max(0, ext.seen - (it.first + j) * kPromptKeys), g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
                     mbar_wait(bar(Plan::look(k, g)), (look >> at) & 1u, &s_failed);
                     look ^= 1u << at;
                     const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>((tile0 + 2 * j + 1) % Plan::kStages) * Plan::kTileBytes;
@@ -760,20 +763,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     constexpr uint32_t kOne = (0x8000u - F16Kind<T>::kExponent) * 0x10001u;
                     const auto carries = [&](uint32_t w) { return (w & kMask) + kOne; };
                     uint32_t any = 0;
-#pragma unroll 8
-                    for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
-                        if ((c % 1024) / 8 < rows) {
-                            const uint4 w = lds128(where(c));
+#pragma unroll 4
+                    for (int c = 8 * row0 + t; c < 8 * rows; c += 64)
+#pragma unroll
+                        for (int hh = 0; hh < Plan::kHalves; ++hh) {
+                            const uint4 w = lds128(where(c + 1024 * hh));
                             any |= carries(w.x) | carries(w.y) | carries(w.z) | carries(w.w);
                         }
-                    }
                     for (int c = 8 * rows + t; c < 8 * ((rows + 15) & ~15); c += 64)
 #pragma unroll
                         for (int hh = 0; hh < Plan::kHalves; ++hh) sts128(where(c + 1024 * hh), make_uint4(0, 0, 0, 0));
                     if (any & 0x80008000u) {
                         s_poison[k & 1] = 1;
-                        for (int c = t; c < 1024 * Plan::kHalves; c += 64) {
-                            if ((c % 1024) / 8 >= rows) continue;
+                        for (int c = 8 * row0 + t; c < 8 * rows + 1024 * (Plan::kHalves - 1); c += 64) {
+                            if ((c % 1024) / 8 >= rows || (c % 1024) / 8 < row0) continue;
                             const uint4 w = lds128(where(c));
                             uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -844,7 +847,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                     if (!mine) continue;
 #pragma unroll 1
-                    for (int pos = max(ext.guarded, it.first) * kPromptKeys; pos < min(sees, it.end * kPromptKeys); ++pos) {
+                    for (int pos = max(ext.seen, it.first * kPromptKeys); pos < min(sees, it.end * kPromptKeys); ++pos) {
                         const long long row = cache_row(p.cache, it.seq, pos, it.head);
                         if (row < 0) continue;
                         const T *v = static_cast<const T *>(p.cache.v) + row + 16 * q;

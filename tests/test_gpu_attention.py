@@ -651,3 +651,19 @@ def test_scores_that_are_all_minus_infinity_give_zeros():
     for got in (dmm.paged_attention(q, k, v, table, lens), dmm.prompt_attention(q, k, v, table, lens, cu_of([1, 1, 1]))):
         assert bool((got[:2] == 0).all())
         assert check_attention(got[2], want[2], bound[2]) == 4 * 128
+
+
+@pytest.mark.parametrize("new,past,at", [(40, 9000, 8999), (40, 9000, 9000), (40, 9000, 9001), (40, 200, 200), (40, 200, 130), (9, 0, 0), (300, 100, 100)])
+def test_a_value_at_the_edge_of_what_every_row_sees(new, past, at):
+    # infinite in one column: the rows that see it have the infinity there (or NaN), each once, and nothing else changes
+    gen = generator(28)
+    k, v, table, lens = make_cache(gen, [new + past], 2, 64, 16, FP16)
+    q = torch.randn((new, 8, 64), generator=gen, device="cuda").to(FP16)
+    want, bound = attention(q, k, v, table, lens, cu_of([new]))
+    v[int(table[0, at // 16]), 1, at % 16, 5] = math.inf
+    got = dmm.prompt_attention(q, k, v, table, lens, cu_of([new]))
+    seen = torch.arange(past, past + new, device="cuda") >= at
+    assert not bool(torch.isfinite(got[seen][:, 4:, 5]).any()) and bool(seen.any())
+    got[seen, 4:, 5] = 0
+    want[seen, 4:, 5] = 0
+    assert check_attention(got, want, bound) == got.numel()
