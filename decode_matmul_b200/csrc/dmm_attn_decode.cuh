@@ -42,17 +42,19 @@ struct DecodeParams {
 // kN: column tiles of 8 queries.
 template <int D, int kN>
 struct DecodePlan {
-    static constexpr int kStages = (D == 128 ? 3 : 6) - (kN == 2 ? D == 128 ? 1 : 2 : 0);
+    static constexpr int kStages = (D == 128 ? 3 : 5) - (kN == 2 ? 1 : 0);
     static constexpr uint32_t kRowBytes = 2 * D;
     static constexpr uint32_t kUnitBytes = kUnitKeys * kRowBytes;  // of K, and again of V
     static constexpr uint32_t kWarpBytes = kStages * 2 * kUnitBytes;
     // A part of a segment: weighted sums of values (a row per query, padded against bank conflicts), then maximum and sum of each.
     static constexpr int kRows = 8 * kN, kPad = D + 4;
     static constexpr int kPartFloats = kRows * (kPad + 2);
-    // the rings, and the queries of two segments per warp beside them; a warp's last part takes the place of its ring
+    // The rings, and beside them the queries of the units under way, which may be as many segments (the present one's are in registers); a
+    // warp's last part takes the place of its ring.
+    static constexpr int kQPlaces = kStages > 2 ? kStages - 1 : 2;
     static constexpr uint32_t kQBytes = kRows * kRowBytes;
     static constexpr uint32_t kQ = kDecodeWarps * kWarpBytes;
-    static constexpr uint32_t kBytes = kQ + kDecodeWarps * 2 * kQBytes;
+    static constexpr uint32_t kBytes = kQ + kDecodeWarps * kQPlaces * kQBytes;
     static_assert(kPartFloats * 4 <= kWarpBytes, "a part fits into a ring");
     static_assert(kBytes <= 227 * 1024 - 1024, "shared memory");
 };
@@ -241,15 +243,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
         bool fresh_load = true;                // the next of them is the first of its segment
         const int32_t *table = p.cache.page_table + load.seq * p.cache.table_stride;
         int page = load.len > 0 ? table[(load.unit * kUnitKeys) >> p.cache.page_shift] : 0;
-        // The queries of a segment come with its first unit here, into one of two places in turn: at most two segments' are
-        // under way, since those of the present one are in registers by then.
-        const uint32_t q_place = smem_u32(smem_raw) + Plan::kQ + warp * 2 * Plan::kQBytes;
+        // the queries of a segment come with its first unit here, into the places in turn
+        const uint32_t q_place = smem_u32(smem_raw) + Plan::kQ + warp * Plan::kQPlaces * Plan::kQBytes;
         int q_load = 0, q_use = 0;
         const auto issue_q = [&]() {
             const int r0 = load.tile * Plan::kRows;
             const T *q = static_cast<const T *>(p.q) + load.seq * p.q_ld + (static_cast<long long>(load.head) * p.group + r0) * D + piece * 8;
             const uint32_t dst = q_place + q_load * Plan::kQBytes;
-            q_load ^= 1;
+            if (++q_load == Plan::kQPlaces) q_load = 0;
 #pragma unroll
             for (int i = 0; i < Plan::kRows / kRowsAtOnce; ++i) {
                 const int row = row0 + i * kRowsAtOnce;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             }
             if (n >= 0 && fresh) {
                 const uint32_t q = q_place + q_use * Plan::kQBytes;
-                q_use ^= 1;
+                if (++q_use == Plan::kQPlaces) q_use = 0;
 #pragma unroll
                 for (int t = 0; t < kN; ++t) {
 #pragma unroll
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                 }
                 fresh = false;
                 have = 0;
-                __syncwarp();  // (the next queries but one come to this place)
+                __syncwarp();  // (other queries come to this place)
             }
             if (left > 0) issue(fill);
             cp_async_commit();

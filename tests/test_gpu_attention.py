@@ -667,3 +667,18 @@ def test_a_value_at_the_edge_of_what_every_row_sees(new, past, at):
     got[seen, 4:, 5] = 0
     want[seen, 4:, 5] = 0
     assert check_attention(got, want, bound) == got.numel()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("group", [1, 8, 16, 40])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_many_sequences_of_a_few_tokens(D, group, dtype):
+    # a warp has a new sequence, key head and queries with every 16 keys, or with every second and third
+    gen = generator(29)
+    lens_ = [(7 * i) % 17 for i in range(150)] + [(11 * i) % 49 for i in range(150)] + [16, 32, 1, 0, 500, 3, 17]
+    k, v, table, lens = make_cache(gen, lens_, 4, D, 16, dtype)
+    q = torch.randn((len(lens_), 4 * group, D), generator=gen, device="cuda").to(dtype)
+    want, bound = attention(q, k, v, table, lens, None)
+    got = dmm.paged_attention(q, k, v, table, lens)
+    assert check_attention(got, want, bound) == got.numel()
+    assert torch.equal(got, dmm.paged_attention(q, k, v, table, lens)) and dmm.status() == 0
