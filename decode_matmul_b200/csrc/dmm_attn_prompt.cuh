@@ -22,8 +22,8 @@
 // each other: 128 scores a thread, the maximum, the exponentials, P V and the next S take about 3600 cycles, and two tiles
 // of a CTA are all that tensor memory holds (2 x (128 + 128) columns of 512).  Of it the weights' hand-over is cut in two, so that
 // P V begins when 80 of 128 keys have theirs.
-// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 915 us (1.20 PFLOP/s, 72 % of what a dense product reaches; tensor pipe
-// 58 % busy, exponentials 59 %), 2048 tokens 79 us (0.87 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
+// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 907 us (1.21 PFLOP/s, 73 % of what a dense product reaches; tensor pipe
+// 58 % busy, exponentials 59 %), 2048 tokens 77 us (0.89 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
 // guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.
 #pragma once
 
