@@ -64,18 +64,19 @@ struct PromptPlan {
     // Barriers, in the order of their use for an item.  What not every item uses twice in a row has a phase of its own, which its users
     // count; the guard's come in two sets that the items use in turn.
     static constexpr int kBarItem = 0, kBarItemFree = 2, kBarNext = 4, kBarQ = 5, kBarQFree = 7, kBarFull = 9, kBarEmpty = kBarFull + kStages,
-                         kBarS = kBarEmpty + kStages, kBarP = kBarS + 2, kBarO = kBarP + 4, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
+                         kBarS = kBarEmpty + kStages, kBarDone = kBarS + 2, kBarSFree = kBarDone + 2, kBarP = kBarSFree + 1, kBarO = kBarP + 4, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
                          kBarGuard = kBarLook + 2 * kMostGuarded, kNumBars = kBarGuard + 2 * kMostGuarded;
     __device__ static constexpr int phase_bit(int item, int tile) { return (item & 1) * kMostGuarded + tile; }
     __device__ static constexpr int look(int item, int tile) { return kBarLook + phase_bit(item, tile); }
     __device__ static constexpr int guard(int item, int tile) { return kBarGuard + phase_bit(item, tile); }
     __device__ static constexpr uint32_t arrivals(int bar) {
         if (bar >= kBarItemFree && bar < kBarNext) return 11;  // every warp but the one that finds the items
-        if ((bar >= kBarP && bar < kBarO) || (bar >= kBarOFree && bar < kBarLook)) return 4;
+        if ((bar >= kBarSFree && bar < kBarO) || (bar >= kBarOFree && bar < kBarLook)) return 4;
         return bar >= kBarGuard ? 2 : 1;
     }
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 64 + 1024;  // (the last: alignment)
-    static constexpr uint32_t kS = 0, kO = 256;       // tensor memory columns: S of tile i at 128 i, O at 256 + D i
+    // tensor memory columns: P of tile i at 64 i, S of either tile, O of tile i at 256 + D i
+    static constexpr uint32_t kP = 0, kS = 128, kO = 256;
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *tmap, int x, int y, int z, int w, uint32_t bar) {
@@ -350,9 +351,11 @@ __device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&u)[16]) 
 // l: their sum so far.
 template <class T, int D>
 struct SoftmaxRow {
-    uint32_t s_at, o_at;   // tensor memory of S (then P) and O
+    uint32_t s_at, p_at, o_at;  // tensor memory of S, P and O
     float c;               // weights are 2^(c S - c m)
-    uint32_t bar;          // barriers of the two parts of P
+    uint32_t bar, bar_free, bar_done;  // barriers of the two parts of P, of S when it has been read, and of the products before
+    uint32_t done;         // phase of the last
+    volatile int *failed;
     int sees;              // keys of the tile that the row sees
     bool begun;            // O has a sum already
 
@@ -373,6 +376,9 @@ struct SoftmaxRow {
             if (half == 1) {
                 tmem_wait_ld32(u + 64);
                 tmem_wait_ld32(u + 96);
+                tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(bar_free);  // (the other tile's scores come to this place)
             }
             if constexpr (kMasked) {
 #pragma unroll
@@ -386,6 +392,10 @@ struct SoftmaxRow {
             }
         }
         const float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
+        if (begun) {  // the products of the tile before have read P and are in O
+            mbar_wait(bar_done, done, failed);
+            tc_fence_after();
+        }
         const bool rise = top > m && (m == -INFINITY || (top - m) * c > 8.0f);
         if (__any_sync(0xffffffffu, rise)) {
             const float to = rise ? top : m, f = m == -INFINITY ? 0.0f : exp2_fast((m - to) * c);
@@ -417,7 +427,7 @@ struct SoftmaxRow {
                 sums[x % 4] = add2(sums[x % 4], pair32(y.x, y.y));
                 w[x] = pack16<T>(y.x, y.y);
             }
-            tmem_st8(s_at + 8 * q, w);
+            tmem_st8(p_at + 8 * q, w);
             if (q + 1 == kPromptEarly || q == 7) {  // the products of these keys can begin
                 tmem_wait_st();
                 tc_fence_before();
@@ -638,107 +648,110 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             // V, the distance from one 64 columns to the next
             constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
             const auto lo = [&](uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); };
-            // the ring's next tile: where it is, and the wait for it
-            int stage = 0;
-            uint32_t parity = 0;
             const auto place = [&](int s) { return smem + Plan::kRing + static_cast<uint32_t>(s) * Plan::kTileBytes; };
-            const auto step = [&]() {
-                if (++stage == Plan::kStages) {
-                    stage = 0;
-                    parity ^= 1u;
-                }
-            };
-            const auto scores = [&](int i, int s) {
-                const uint32_t a = lo(smem + Plan::kQ + i * Plan::kTileBytes, 16), b = lo(place(s), 16);
-                if (leader) {
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (k / 4) * (Plan::kHalfBytes >> 4) + (k % 4) * 2;
-                        mma_ss_f16(tmem + Plan::kS + 128 * i, a + off, kHi, b + off, kHi, id_s, k > 0);
+            // A place of the ring: keys and values have every second one.
+            struct Ring {
+                int stage;
+                uint32_t parity;
+                __device__ __forceinline__ void step() {
+                    stage += 2;
+                    if (stage >= Plan::kStages) {
+                        stage -= Plan::kStages;
+                        parity ^= 1u;
                     }
-                    tc_commit(bar(Plan::kBarS + i));
                 }
             };
-            uint32_t q_full = 0, p_full = 0, o_free = 0, guard = 0;  // bits: phases
+            Ring keys = {0, 0}, values = {1, 0};
+            uint32_t q_full = 0, p_full = 0, o_free = 0, guard = 0, s_count = 0;  // bits: phases
             bool o_used[2] = {false, false};
             for (int k = 0;; ++k) {
                 const PromptItem it = item_of(k);
                 if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
-                if (ext.all > 0) {
-                    mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (ext.tiles[i] > 0) {
-                            mbar_wait(bar(Plan::kBarQ + i), (q_full >> i) & 1u, &s_failed);
-                            q_full ^= 1u << i;
-                            tc_fence_after();
-                            scores(i, stage);
-                            if (leader && ext.tiles[i] == 1) tc_commit(bar(Plan::kBarQFree + i));
-                        }
-                    if (leader) tc_commit(bar(Plan::kBarEmpty + stage));
-                    step();
-                }
-                bool v_seen = false, k_seen = false;  // the next values and keys were seen to be there
-                for (int j = 0; j < ext.all; ++j) {
-                    if (!v_seen) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
-                    if (it.first + j >= ext.guarded) {
-                        const int g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
-                        mbar_wait(bar(Plan::guard(k, g)), (guard >> at) & 1u, &s_failed);
-                        guard ^= 1u << at;
+                // Scores and products go in the order (tile 0, key tile 0), (tile 1, 0), (0, 1), (1, 1), ...; the scores of two are asked
+                // for before the products of the first, and then always the next ones behind those of one more: they are there when
+                // a tile's softmax has done with the scores before.
+                int si = ext.tiles[0] > 0 ? 0 : 1, sj = 0, pi = si, pj = 0;
+                const auto next = [&](int &i, int &j) {  // false: there is no other for this key tile
+                    if (i == 0 && j < ext.tiles[1]) {
+                        i = 1;
+                        return true;
                     }
-                    const int v_stage = stage;
-                    const uint32_t v = lo(place(v_stage), Plan::kHalfBytes);
-                    step();
-                    if (j + 1 < ext.all && !k_seen) mbar_wait(bar(Plan::kBarFull + stage), parity, &s_failed);
-                    v_seen = k_seen = false;
-                    bool k_there = false;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        // (a look at a barrier takes a while even when its phase is complete, and the tensor cores have few products in
-                        // store: the next tiles are looked for before the last products of this round are issued)
-                        if (i == 1 && j + 1 < ext.all) {
-                            const int s1 = stage + 1 == Plan::kStages ? 0 : stage + 1, s2 = s1 + 1 == Plan::kStages ? 0 : s1 + 1;
-                            v_seen = mbar_test(bar(Plan::kBarFull + s1), parity ^ (s1 < stage ? 1u : 0u));
-                            k_seen = j + 2 < ext.all && mbar_test(bar(Plan::kBarFull + s2), parity ^ (s2 < stage ? 1u : 0u));
-                        }
-                        if (j < ext.tiles[i]) {
-                            if (j == 0) {  // the epilogue before has read O
-                                if (o_used[i]) {
-                                    mbar_wait(bar(Plan::kBarOFree + i), (o_free >> i) & 1u, &s_failed);
-                                    o_free ^= 1u << i;
-                                }
-                                o_used[i] = true;
-                            }
-                            // (the last tile: only the 16 keys at a time that some row sees)
-                            const int steps = min(8, (ext.most[i] - (it.first + j) * kPromptKeys + 15) / 16);
-                            const uint32_t begun = j > 0 ? 1u : 0u;
-#pragma unroll
-                            for (int part = 0; part < 2; ++part) {
-                                mbar_wait(bar(Plan::kBarP + 2 * i + part), (p_full >> i) & 1u, &s_failed);
-                                tc_fence_after();
-                                if (leader) {
-#pragma unroll
-                                    for (int n = part == 0 ? 0 : kPromptEarly; n < (part == 0 ? kPromptEarly : 8); ++n)
-                                        if (n < steps)
-                                            mma_ts_f16_words(tmem + Plan::kO + D * i, tmem + Plan::kS + 128 * i + 8 * n, v + n * (2048u >> 4), kHi, kIdO, n > 0 ? 1u : begun);
-                                }
-                                __syncwarp();
-                            }
-                            p_full ^= 1u << i;
-                            if (leader && j + 1 == ext.tiles[i]) tc_commit(bar(Plan::kBarO + i));
-                        }
-                        if (j + 1 < ext.tiles[i]) {
-                            k_there = true;
-                            scores(i, stage);
-                            if (leader && j + 2 == ext.tiles[i]) tc_commit(bar(Plan::kBarQFree + i));
-                        }
+                    ++j;
+                    i = j < ext.tiles[0] ? 0 : 1;
+                    return false;
+                };
+                bool new_keys = true, new_values = true;
+                const auto scores = [&]() {
+                    if (sj >= ext.all) return;
+                    if (new_keys) mbar_wait(bar(Plan::kBarFull + keys.stage), keys.parity, &s_failed);
+                    if (sj == 0) {
+                        mbar_wait(bar(Plan::kBarQ + si), (q_full >> si) & 1u, &s_failed);
+                        q_full ^= 1u << si;
                     }
+                    if (s_count > 0) mbar_wait(bar(Plan::kBarSFree), (s_count - 1) & 1u, &s_failed);
+                    ++s_count;
+                    tc_fence_after();
+                    const uint32_t a = lo(smem + Plan::kQ + si * Plan::kTileBytes, 16), b = lo(place(keys.stage), 16);
                     if (leader) {
-                        tc_commit(bar(Plan::kBarEmpty + v_stage));
-                        if (k_there) tc_commit(bar(Plan::kBarEmpty + stage));
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d) {
+                            const uint32_t off = (d / 4) * (Plan::kHalfBytes >> 4) + (d % 4) * 2;
+                            mma_ss_f16(tmem + Plan::kS, a + off, kHi, b + off, kHi, id_s, d > 0);
+                        }
+                        tc_commit(bar(Plan::kBarS + si));
+                        if (sj + 1 == (si == 0 ? ext.tiles[0] : ext.tiles[1])) tc_commit(bar(Plan::kBarQFree + si));
                     }
-                    if (k_there) step();
+                    __syncwarp();
+                    new_keys = !next(si, sj);
+                    if (new_keys) {
+                        if (leader) tc_commit(bar(Plan::kBarEmpty + keys.stage));
+                        __syncwarp();
+                        keys.step();
+                    }
+                };
+                scores();
+                scores();
+                if (ext.tiles[0] > 0 && ext.tiles[1] > 0) scores();
+                while (pj < ext.all) {
+                    if (new_values) {
+                        mbar_wait(bar(Plan::kBarFull + values.stage), values.parity, &s_failed);
+                        if (it.first + pj >= ext.guarded) {
+                            const int g = it.first + pj - ext.guarded, at = Plan::phase_bit(k, g);
+                            mbar_wait(bar(Plan::guard(k, g)), (guard >> at) & 1u, &s_failed);
+                            guard ^= 1u << at;
+                        }
+                    }
+                    if (pj == 0) {  // the epilogue before has read O
+                        if (pi == 0 ? o_used[0] : o_used[1]) {
+                            mbar_wait(bar(Plan::kBarOFree + pi), (o_free >> pi) & 1u, &s_failed);
+                            o_free ^= 1u << pi;
+                        }
+                        (pi == 0 ? o_used[0] : o_used[1]) = true;
+                    }
+                    // (the last tile: only the 16 keys at a time that some row sees)
+                    const int steps = min(8, ((pi == 0 ? ext.most[0] : ext.most[1]) - (it.first + pj) * kPromptKeys + 15) / 16);
+                    const uint32_t begun = pj > 0 ? 1u : 0u, v = lo(place(values.stage), Plan::kHalfBytes);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        mbar_wait(bar(Plan::kBarP + 2 * pi + part), (p_full >> pi) & 1u, &s_failed);
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (int n = part == 0 ? 0 : kPromptEarly; n < (part == 0 ? kPromptEarly : 8); ++n)
+                                if (n < steps) mma_ts_f16_words(tmem + Plan::kO + D * pi, tmem + Plan::kP + 64 * pi + 8 * n, v + n * (2048u >> 4), kHi, kIdO, n > 0 ? 1u : begun);
+                        }
+                        __syncwarp();
+                    }
+                    p_full ^= 1u << pi;
+                    if (leader) tc_commit(bar((pj + 1 == (pi == 0 ? ext.tiles[0] : ext.tiles[1]) ? Plan::kBarO : Plan::kBarDone) + pi));
+                    new_values = !next(pi, pj);
+                    if (new_values) {
+                        if (leader) tc_commit(bar(Plan::kBarEmpty + values.stage));
+                        values.step();
+                    }
+                    __syncwarp();
+                    scores();
                 }
                 item_done(k);
             }
@@ -800,10 +813,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         // =============================== softmax ===============================
         const int i = warp / 4, r = threadIdx.x % 128, magic = 65536 / p.group + 1, tok = r * magic >> 16;  // (r / group, for r < 128)
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp % 4)) << 16);
-        const uint32_t s_at = lanes + Plan::kS + 128 * i, o_at = lanes + Plan::kO + D * i;
+        const uint32_t s_at = lanes + Plan::kS, p_at = lanes + Plan::kP + 64 * i, o_at = lanes + Plan::kO + D * i;
         // (the products have the sign of the scale; times 2^-149 every finite score is as good as 0, and a hidden one stays -infinity)
         const float c = p.scale == 0.0f ? __uint_as_float(1u) : fabsf(p.scale) * 1.4426950408889634f;
-        uint32_t s_full = 0, o_full = 0;  // phases
+        uint32_t s_full = 0, o_full = 0, done = 0;  // phases
         for (int k = 0;; ++k) {
             const PromptItem it = item_of(k);
             if (it.seq < 0) break;
@@ -818,7 +831,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
                 s_full ^= 1u;
                 tc_fence_after();
-                const SoftmaxRow<T, D> row = {s_at, o_at, c, bar(Plan::kBarP + 2 * i), sees - (it.first + j) * kPromptKeys, j > 0};
+                const SoftmaxRow<T, D> row = {s_at, p_at, o_at, c, bar(Plan::kBarP + 2 * i), bar(Plan::kBarSFree), bar(Plan::kBarDone + i), done, &s_failed,
+                                              sees - (it.first + j) * kPromptKeys, j > 0};
+                if (j > 0) done ^= 1u;
                 if (j < free)
                     row.template step<false>(m, l);
                 else
