@@ -6,7 +6,8 @@
 // A CTA has two tiles of 128 query rows of one key head and one sequence, so that the tensor cores work for one tile while
 // the softmax of the other runs.  The rows of a tile are (token, query head of the group): all the heads that share a
 // key head read its tile once, and a tile spans few tokens, so little of the causal triangle's edge is computed in vain.
-// Tensor memory holds S of both tiles (2 x 128 columns; P, in 16 bits, takes the place of the first half of its S) and O of both.
+// Tensor memory holds O of both tiles (2 x D columns), P of both in 16 bits (2 x 64) and one S (128), which the tiles use in turn: a tile's
+// scores stay there only until its softmax has them in registers, and the next ones are there when it has done with these.
 //   warps 0..3, 4..7   softmax of tile 0, 1: a thread has a row
 //   warp 8             MMA issue (one elected lane)
 //   warp 9             TMA loads: Q, then K_0, V_0, K_1, ...; a tile of keys is one box per page
@@ -18,13 +19,13 @@
 // cores take them; sums, maxima and O are fp32.
 //
 // Bound: 4 D operations for each (row, key) on the tensor cores, 2048 cycles for two tiles of 128 x 128 at D = 128, and as many
-// cycles for their 32768 exponentials (16 a cycle).  Neither is reached, because S, the weights and P V of one tile depend on
-// each other: 128 scores a thread, the maximum, the exponentials, P V and the next S take about 3600 cycles, and two tiles
-// of a CTA are all that tensor memory holds (2 x (128 + 128) columns of 512).  Of it the weights' hand-over is cut in two, so that
-// P V begins when 80 of 128 keys have theirs.
-// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 907 us (1.21 PFLOP/s, 73 % of what a dense product reaches; tensor pipe
-// 58 % busy, exponentials 59 %), 2048 tokens 77 us (0.89 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
-// guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.
+// cycles for their 32768 exponentials (16 a cycle).  Neither is reached: a step of a tile's softmax takes some 2000 cycles of a warp (scores
+// into registers, the maximum, the exponentials, of which two tiles' share the unit) and waits some 800 for products, and two tiles of
+// a CTA are all that tensor memory holds.
+// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 851 us (1.29 PFLOP/s, 78 % of what a dense product reaches), 2048 tokens 74 us
+// (0.93 PFLOP/s): every item has a beginning (its first keys' way
+// from HBM, the guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.  Under a load of
+// some seconds the clock falls to 1.6 GHz at the power cap, and 8192 tokens take 970 to 990 us.
 #pragma once
 
 #include "dmm_attn_common.cuh"
@@ -46,8 +47,6 @@ struct PromptParams {
 
 constexpr int kPromptThreads = 384;
 constexpr int kPromptKeys = 128;  // keys of a tile
-constexpr int kPromptEarly = 5;   // of the 8 steps of 16 keys that P V takes: those that begin before the rest of P is there (2 to 7
-                                  // measure within 1 %, 8 would be none)
 
 // Key tiles in which rows of a pair of tiles end: they are 256 tokens at most.
 constexpr int kMostGuarded = 3;
@@ -64,7 +63,7 @@ struct PromptPlan {
     // Barriers, in the order of their use for an item.  What not every item uses twice in a row has a phase of its own, which its users
     // count; the guard's come in two sets that the items use in turn.
     static constexpr int kBarItem = 0, kBarItemFree = 2, kBarNext = 4, kBarQ = 5, kBarQFree = 7, kBarFull = 9, kBarEmpty = kBarFull + kStages,
-                         kBarS = kBarEmpty + kStages, kBarDone = kBarS + 2, kBarSFree = kBarDone + 2, kBarP = kBarSFree + 1, kBarO = kBarP + 4, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
+                         kBarS = kBarEmpty + kStages, kBarDone = kBarS + 2, kBarSFree = kBarDone + 2, kBarP = kBarSFree + 1, kBarO = kBarP + 2, kBarOFree = kBarO + 2, kBarLook = kBarOFree + 2,
                          kBarGuard = kBarLook + 2 * kMostGuarded, kNumBars = kBarGuard + 2 * kMostGuarded;
     __device__ static constexpr int phase_bit(int item, int tile) { return (item & 1) * kMostGuarded + tile; }
     __device__ static constexpr int look(int item, int tile) { return kBarLook + phase_bit(item, tile); }
@@ -353,7 +352,7 @@ template <class T, int D>
 struct SoftmaxRow {
     uint32_t s_at, p_at, o_at;  // tensor memory of S, P and O
     float c;               // weights are 2^(c S - c m)
-    uint32_t bar, bar_free, bar_done;  // barriers of the two parts of P, of S when it has been read, and of the products before
+    uint32_t bar, bar_free, bar_done;  // barriers of P, of S when it has been read, and of the products before
     uint32_t done;         // phase of the last
     volatile int *failed;
     int sees;              // keys of the tile that the row sees
@@ -428,13 +427,11 @@ struct SoftmaxRow {
                 w[x] = pack16<T>(y.x, y.y);
             }
             tmem_st8(p_at + 8 * q, w);
-            if (q + 1 == kPromptEarly || q == 7) {  // the products of these keys can begin
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if ((threadIdx.x & 31) == 0) mbar_arrive(bar + (q == 7 ? 8u : 0u));
-            }
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
         const float2 sum = unpair32(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
         l += sum.x + sum.y;
     }
@@ -732,18 +729,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     // (the last tile: only the 16 keys at a time that some row sees)
                     const int steps = min(8, ((pi == 0 ? ext.most[0] : ext.most[1]) - (it.first + pj) * kPromptKeys + 15) / 16);
                     const uint32_t begun = pj > 0 ? 1u : 0u, v = lo(place(values.stage), Plan::kHalfBytes);
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        mbar_wait(bar(Plan::kBarP + 2 * pi + part), (p_full >> pi) & 1u, &s_failed);
-                        tc_fence_after();
-                        if (leader) {
-#pragma unroll
-                            for (int n = part == 0 ? 0 : kPromptEarly; n < (part == 0 ? kPromptEarly : 8); ++n)
-                                if (n < steps) mma_ts_f16_words(tmem + Plan::kO + D * pi, tmem + Plan::kP + 64 * pi + 8 * n, v + n * (2048u >> 4), kHi, kIdO, n > 0 ? 1u : begun);
-                        }
-                        __syncwarp();
-                    }
+                    mbar_wait(bar(Plan::kBarP + pi), (p_full >> pi) & 1u, &s_failed);
                     p_full ^= 1u << pi;
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                            if (n < steps) mma_ts_f16_words(tmem + Plan::kO + D * pi, tmem + Plan::kP + 64 * pi + 8 * n, v + n * (2048u >> 4), kHi, kIdO, n > 0 ? 1u : begun);
+                    }
+                    __syncwarp();
                     if (leader) tc_commit(bar((pj + 1 == (pi == 0 ? ext.tiles[0] : ext.tiles[1]) ? Plan::kBarO : Plan::kBarDone) + pi));
                     new_values = !next(pi, pj);
                     if (new_values) {
@@ -831,7 +825,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 mbar_wait(bar(Plan::kBarS + i), s_full, &s_failed);
                 s_full ^= 1u;
                 tc_fence_after();
-                const SoftmaxRow<T, D> row = {s_at, p_at, o_at, c, bar(Plan::kBarP + 2 * i), bar(Plan::kBarSFree), bar(Plan::kBarDone + i), done, &s_failed,
+                const SoftmaxRow<T, D> row = {s_at, p_at, o_at, c, bar(Plan::kBarP + i), bar(Plan::kBarSFree), bar(Plan::kBarDone + i), done, &s_failed,
                                               sees - (it.first + j) * kPromptKeys, j > 0};
                 if (j > 0) done ^= 1u;
                 if (j < free)
