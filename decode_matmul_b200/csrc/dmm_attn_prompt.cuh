@@ -22,10 +22,10 @@
 // cycles for their 32768 exponentials (16 a cycle).  Neither is reached: a step of a tile's softmax takes some 2000 cycles of a warp (scores
 // into registers, the maximum, the exponentials, of which two tiles' share the unit) and waits some 800 for products, and two tiles of
 // a CTA are all that tensor memory holds.
-// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 851 us (1.29 PFLOP/s, 78 % of what a dense product reaches), 2048 tokens 74 us
-// (0.93 PFLOP/s): every item has a beginning (its first keys' way
-// from HBM, the guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.  Under a load of
-// some seconds the clock falls to 1.6 GHz at the power cap, and 8192 tokens take 970 to 990 us.
+// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 850 us (1.29 PFLOP/s, 78 % of what a dense product reaches; tensor
+// pipe 65 % busy, exponentials 65 %), 2048 tokens 73 us (0.94 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
+// guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.  Under a load of some seconds
+// the clock falls to 1.6 GHz at the power cap, and 8192 tokens take 970 to 990 us.
 #pragma once
 
 #include "dmm_attn_common.cuh"
@@ -171,7 +171,7 @@ struct PromptItem {
 };
 
 constexpr int kPromptItem = 2;
-constexpr float kPromptJoin = 4.0f, kPromptLeast = 0.28f;  // 0.28 = sqrt(0.15 us a part in the join / 1.9 us a key tile)
+constexpr float kPromptJoin = 6.0f, kPromptLeast = 0.28f;  // 0.28 = sqrt(0.15 us a part in the join / 1.8 us a key tile)
 
 // The sequences of one lane each, from b0 on; by a warp.
 struct PromptSeqs {
@@ -205,9 +205,9 @@ __device__ __forceinline__ float warp_sum(float x) {
 //               kPromptJoin key tiles, and longer the more parts an item has: shares are no smaller than kPromptLeast
 //               times the square root of the longest item, and CTAs without one stay idle.
 // Which of the two ends sooner is estimated: whole items end with the longest, or half of the shortest of a sequence (on
-// average over the work) behind an even share.  B200, whole items against even shares: a prompt of 2048 tokens 81 us against
-// 140, of 8192 927 against 1818 (an item counts as the longest of its sequence); four chunks of 33 to 512 tokens behind 511 to 16384
-// 257 against 198; 16 tokens of 8 heads behind 16384 215 against 37.
+// average over the work) behind an even share.  B200, whole items against even shares: a prompt of 2048 tokens 74 us against
+// 131, of 8192 869 against 1660 (an item counts as the longest of its sequence), of 1024 with 8 heads 23 against 28; four chunks of 33 to
+// 512 tokens behind 511 to 16384 238 against 185; 16 tokens of 8 heads behind 16384 164 against 34.
 struct PromptShare {
     int each, more, all;
     __device__ __forceinline__ int begin(int x) const { return min(each * x + min(x, more), all); }
