@@ -10,7 +10,7 @@
 //
 // Bound: bytes, 4 (fp32) or 2 read and 2 written for each value.  B200, graph: 2048 tokens of 64 + 16 heads of 128, fp32 in,
 // 22.0 us (5.7 TB/s, 88 % of what a copy reaches); 8164 tokens of prompts of many lengths 81 us (6.2 TB/s, 94 %).  One token
-// takes 2.1 us, a launch and three dependent loads: its sequence's length and page and the row itself.
+// takes 2.9 us (2.3 when all of it is in L2), a launch and three dependent loads: its sequence's length and page and the row itself.
 #pragma once
 
 #include "dmm_attn_common.cuh"
@@ -130,8 +130,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
 template <class TIn, class T, int D>
 inline int launch_append_typed(const AppendParams &p, int num_sms, bool pdl, cudaStream_t stream) {
     const int units = (p.heads + 2 * p.cache.kv_heads) * (D / 16);
-    // Few tokens: a thread takes one unit, so that all of the GPU loads at once (one token of 80 heads 2.1 us against 3.6 with one
-    // block for the token, 32 tokens of 96 heads 2.6 against 4.3); many: a block keeps its token, whose sines and cosines it works out
+    // Few tokens: a thread takes one unit, so that all of the GPU loads at once (with all of it in L2 one token of 80 heads 2.1 us
+    // against 3.6 with one block for the token, 32 tokens of 96 heads 2.6 against 4.3); many: a block keeps its token, whose sines and cosines it works out
     // once (8164 tokens 81 us against 92).
     int parts = (units + kAppendThreads - 1) / kAppendThreads;
     if (static_cast<long long>(parts) * p.tokens > 16ll * num_sms) parts = 1;

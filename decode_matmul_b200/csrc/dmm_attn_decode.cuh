@@ -17,7 +17,7 @@
 //
 // Bound: bytes, 4 head_dim for every token and key head.  Two units of 8 KB in flight beside the present one for each of 8 warps keep 128 KB
 // under way on every SM, more than HBM's latency asks for.  B200, graph, fp16, heads of 128: 32 sequences with 32 key heads, 405 MB, 72 us (5.6 TB/s,
-// 86 % of what a copy reaches); 16 sequences of 64 heads on 8, 84 MB, 24.2 us; one sequence of 4096, 17 MB, 9.8 us.  What is not
+// 86 % of what a copy reaches); 16 sequences of 64 heads on 8, 84 MB, 24.2 us; one sequence of 4096, 17 MB, 11.6 us (9.8 from L2).  What is not
 // bytes is 8 to 10 us a call: lengths, page numbers and keys are dependent loads, the parts are joined twice, and two kernels start.
 #pragma once
 

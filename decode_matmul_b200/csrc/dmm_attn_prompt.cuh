@@ -22,8 +22,8 @@
 // cycles for their 32768 exponentials (16 a cycle).  Neither is reached: a step of a tile's softmax takes some 2000 cycles of a warp (scores
 // into registers, the maximum, the exponentials, of which two tiles' share the unit) and waits some 800 for products, and two tiles of
 // a CTA are all that tensor memory holds.
-// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 850 us (1.29 PFLOP/s, 78 % of what a dense product reaches; tensor
-// pipe 65 % busy, exponentials 65 %), 2048 tokens 73 us (0.94 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
+// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 856 us (1.28 PFLOP/s, 77 % of what a dense product reaches; tensor
+// pipe 65 % busy, exponentials 65 %), 2048 tokens 70 us (0.98 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
 // guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.  Under a load of some seconds
 // the clock falls to 1.6 GHz at the power cap, and 8192 tokens take 970 to 990 us.
 #pragma once
@@ -205,7 +205,7 @@ __device__ __forceinline__ float warp_sum(float x) {
 //               kPromptJoin key tiles, and longer the more parts an item has: shares are no smaller than kPromptLeast
 //               times the square root of the longest item, and CTAs without one stay idle.
 // Which of the two ends sooner is estimated: whole items end with the longest, or half of the shortest of a sequence (on
-// average over the work) behind an even share.  B200, whole items against even shares: a prompt of 2048 tokens 74 us against
+// average over the work) behind an even share.  B200, whole items against even shares: measured with two copies of a softmax step in the code, a prompt of 2048 tokens 74 us against
 // 131, of 8192 869 against 1660 (an item counts as the longest of its sequence), of 1024 with 8 heads 23 against 28; four chunks of 33 to
 // 512 tokens behind 511 to 16384 238 against 185; 16 tokens of 8 heads behind 16384 164 against 34.
 struct PromptShare {
@@ -887,7 +887,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) tmem_wait_ld(u[q]);
                     }
-#pragma unroll
+#pragma unroll 1
                     for (int e = 0; e < 2; ++e) {
                         const int in_warp = 16 * h + 8 * e + lane / 4, rr = 32 * (warp % 4) + in_warp, t = rr * magic >> 16;
                         const float f = __shfl_sync(0xffffffffu, inv, in_warp);
@@ -899,7 +899,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                                 for (int q = 0; q < D / 32; ++q)
 #pragma unroll
                                     for (int x = 0; x < 4; ++x)
-                                        *reinterpret_cast<uint2 *>(share + rr * D + 32 * q + 8 * x + 2 * (lane % 4)) = make_uint2(u[q][4 * x + 2 * e], u[q][4 * x + 2 * e + 1]);
+                                        *reinterpret_cast<uint2 *>(share + rr * D + 32 * q + 8 * x + 2 * (lane % 4)) = make_uint2(e ? u[q][4 * x + 2] : u[q][4 * x], e ? u[q][4 * x + 3] : u[q][4 * x + 1]);
                             continue;
                         }
 #pragma unroll
@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             uint32_t w[4];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const float2 v = unpair32(mul2(pair32(__uint_as_float(u[q][4 * x + 2 * e]), __uint_as_float(u[q][4 * x + 2 * e + 1])), pair32(f, f)));
+                                const float2 v = unpair32(mul2(pair32(__uint_as_float(e ? u[q][4 * x + 2] : u[q][4 * x]), __uint_as_float(e ? u[q][4 * x + 3] : u[q][4 * x + 1])), pair32(f, f)));
                                 w[x] = pack16<T>(v.x, v.y);
                             }
 #pragma unroll
