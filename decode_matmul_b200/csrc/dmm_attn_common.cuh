@@ -37,6 +37,28 @@ __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t w) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
 }
 
+// Weights of a softmax, which the tensor cores take in the type of the values: 2^(x - m + kRaise<T>) against a running maximum m
+// that is 8 too low at most.  fp16 ends at 2^-25: against a heaviest weight of 1, many light ones beside one heavy key lose their
+// bits or vanish, while the sum of weights has them.  Raised by 7, the heaviest has 2^7 to 2^15, and what vanishes is 2^-32 of it.  (2048 keys
+// beside one that is e^16 times as heavy and has a value of 0: off by 0.48 % on average and 2.3 % at worst without it, 0.017 % and 0.056 % with it.)  The
+// factor is in the sums too, and cancels.  bf16 has the range of fp32.
+template <class T>
+constexpr float kRaise = 0.0f;
+template <>
+constexpr float kRaise<__half> = 7.0f;
+// Two of them rounded to one word.  Scores beyond 2^24, where their products with the scale are rounded to more than 1, can come out above
+// 2^16: not infinite.
+template <class T>
+__device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+    return pack16<T>(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_weights<__half>(float a, float b) {
+    uint32_t w;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+
 // 2^x, off by 2^-22 at most
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

@@ -13,7 +13,9 @@
 // No barrier until a warp has finished.  A segment that a warp has whole is written out by it.  What several warps have of
 // one segment is joined through shared memory, what several CTAs have through the workspace by a second kernel: always in the
 // order of the keys, so that results do not depend on who comes first.
-// The running maximum only moves when it has risen by more than 8 (weights then stay below 2^8).
+// The running maximum only moves when it has risen by more than 8 (weights then stay below 2^8; 2^15 in fp16, see kRaise).  Weights are rounded to
+// the type of the values, as the tensor cores take them: half a step each, in no common direction, which the sum over the keys evens out.
+// Scores, maxima and sums are fp32, the sum of weights that are not rounded.
 //
 // Bound: bytes, 4 head_dim for every token and key head.  Two units of 8 KB in flight beside the present one for each of 8 warps keep 128 KB
 // under way on every SM, more than HBM's latency asks for.  B200, graph, fp16, heads of 128: 32 sequences with 32 key heads, 405 MB, 72 us (5.6 TB/s,
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
                     top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 4));
                     top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 8));
                     top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xffffffffu, top[t][i], 16));
-                    rise |= top[t][i] > m[t][i] + 8.0f;
+                    rise |= top[t][i] - m[t][i] > 8.0f;
                 }
             }
             if (__any_sync(0xffffffffu, rise)) {
@@ -377,11 +379,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1) paged_attention_kernel(c
             for (int t = 0; t < kN; ++t) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[t][i] = exp2_fast(x[t][i] - (m[t][i % 2] == -INFINITY ? 0.0f : m[t][i % 2]));
+                    x[t][i] = exp2_fast(x[t][i] - (m[t][i % 2] == -INFINITY ? 0.0f : m[t][i % 2] - kRaise<T>));
                     l[t][i % 2] += x[t][i];
                 }
-                pf[t][0] = transposed(pack16<T>(x[t][0], x[t][1]));
-                pf[t][1] = transposed(pack16<T>(x[t][2], x[t][3]));
+                pf[t][0] = transposed(pack_weights<T>(x[t][0], x[t][1]));
+                pf[t][1] = transposed(pack_weights<T>(x[t][2], x[t][3]));
             }
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {

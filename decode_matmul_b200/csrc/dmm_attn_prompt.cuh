@@ -15,8 +15,9 @@
 //                      values that are not finite too where a row of the tile must not see them; the epilogue then adds
 //                      them to the rows that do see them.  Only tiles in which a row ends are looked at.
 // O is only brought to a new maximum when that has risen by more than 2^8 (c (max - m) > 8): the weights stay below
-// 2^8, far from overflow, and the quotient O / l is the same.  Weights are rounded to the type of the values, as the tensor
-// cores take them; sums, maxima and O are fp32.
+// 2^8 (2^15 in fp16, see kRaise), far from overflow, and the quotient O / l is the same.  Weights are rounded to the type of the values, as the tensor
+// cores take them: half a step each, in no common direction, which the sum over the keys evens out.  Sums, maxima and O are fp32, l of weights that
+// are not rounded.
 //
 // Bound: 4 D operations for each (row, key) on the tensor cores, 2048 cycles for two tiles of 128 x 128 at D = 128, and as many
 // cycles for their 32768 exponentials (16 a cycle).  Neither is reached: a step of a tile's softmax takes some 2000 cycles of a warp (scores
@@ -412,7 +413,7 @@ struct SoftmaxRow {
                 }
             }
         }
-        const float mc = m == -INFINITY ? 0.0f : -m * c;
+        const float mc = m == -INFINITY ? 0.0f : fmaf(-m, c, kRaise<T>);
         const uint64_t c2 = pair32(c, c), mc2 = pair32(mc, mc);
         uint64_t sums[4] = {};
 #pragma unroll
@@ -424,7 +425,7 @@ struct SoftmaxRow {
                 y.x = exp2_fast(y.x);
                 y.y = exp2_fast(y.y);
                 sums[x % 4] = add2(sums[x % 4], pair32(y.x, y.y));
-                w[x] = pack16<T>(y.x, y.y);
+                w[x] = pack_weights<T>(y.x, y.y);
             }
             tmem_st8(p_at + 8 * q, w);
         }

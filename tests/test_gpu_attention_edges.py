@@ -1,0 +1,70 @@
+"""What the attention operators answer at the edges of what they are given: weights far below the largest, values that are not
+finite inside a sequence, places of a batch that are idle."""
+import math
+
+import pytest
+import torch
+
+import decode_matmul_b200 as dmm
+from attention_reference import attention, check_attention, gather
+from test_gpu_attention import cu_of, generator, make_cache
+
+pytestmark = pytest.mark.gpu
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def tight(bound, v, table, lens, cu, group):
+    """The bound with what subnormal weights may lose put where it belongs: fp16 weights are 2^7 times as large as the reference's
+    bound takes them, the largest is 2^7 at least, and a weight that is rounded to a multiple of 2^-24 is off by 2^-25 at most, which
+    is 2^-32 of the largest."""
+    bound = bound.clone()
+    for b, n in enumerate(lens.tolist()):
+        vmax = gather(v, table[b], n).abs().amax(dim=(1, 2)).repeat_interleave(group)[None, :, None]
+        rows = slice(b, b + 1) if cu is None else slice(int(cu[b]), int(cu[b + 1]))
+        bound[rows] -= n * (2.0 ** -25 - 2.0 ** -32) * vmax
+    return bound
+
+
+@pytest.mark.parametrize("seqs,new,n,kv_heads,group,D", [
+    (1, None, 300, 2, 4, 64), (1, None, 40000, 2, 4, 128),  # a sequence among many warps, each with a maximum of its own
+    (40, None, 300, 32, 1, 128), (40, None, 1500, 32, 1, 64), (80, None, 700, 16, 12, 64),  # a warp has a sequence's key head alone
+    (1, 3, 300, 2, 4, 64), (1, 3, 40000, 2, 4, 128), (1, 600, 2048, 8, 8, 64), (1, 600, 2048, 8, 8, 128), (5, 100, 1000, 16, 2, 128),
+])
+@pytest.mark.parametrize("above", [10.0, 14.0, 16.0])
+def test_a_flat_tail_beside_a_heavy_key(seqs, new, n, kv_heads, group, D, above):
+    """The first key has nearly all of the weight and a value of zero, so the result is what the others add: weights of e^-10 to
+    e^-16 each, which fp16 holds with 10 to no bits when the largest is 1.  new: None for one token of each sequence."""
+    gen = generator(1)
+    k, v, table, lens = make_cache(gen, [n] * seqs, kv_heads, D, 64, FP16)
+    pos = torch.arange(n, device="cuda")
+    for b in range(seqs):
+        page, row = table[b].long()[pos // 64], pos % 64
+        k[page, :, row] = (0.5 * torch.randn((n, kv_heads, D), generator=gen, device="cuda")).to(FP16)
+        k[page, :, row, 0] = 0.0
+        v[page, :, row] = (1.0 + 0.5 * torch.randn((n, kv_heads, D), generator=gen, device="cuda")).to(FP16)
+        k[page[0], :, 0], v[page[0], :, 0] = 0.0, 0.0
+        k[page[0], :, 0, 0] = above
+    q = (0.05 * torch.randn((seqs * (new or 1), kv_heads * group, D), generator=gen, device="cuda")).to(FP16)
+    q[..., 0] = 1.0
+    if new is None:
+        got, cu = dmm.paged_attention(q, k, v, table, lens, 1.0), None
+    else:
+        cu = cu_of([new] * seqs)
+        got = dmm.prompt_attention(q, k, v, table, lens, cu, 1.0)
+    want, bound = attention(q, k, v, table, lens, cu, 1.0)
+    assert check_attention(got, want, tight(bound, v, table, lens, cu, group)) == got.numel()
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_scores_of_millions(dtype):
+    # where a product of a score and the scale is rounded to whole numbers the weights may be any power of 2, but never infinite
+    gen = generator(2)
+    k, v, table, lens = make_cache(gen, [700], 1, 128, 64, dtype)
+    pos = torch.arange(700, device="cuda")
+    k[table[0].long()[pos // 64], :, pos % 64] = 512.0
+    q = torch.full((3, 4, 128), 258.0, dtype=dtype, device="cuda")
+    for i in range(40):  # 258 * 512 * 128 times scales of 0.05 to 12
+        scale = 0.05 * 1.15 ** i
+        want, bound = attention(q, k, v, table, lens, cu_of([3]), scale)
+        for got, rows in ((dmm.prompt_attention(q, k, v, table, lens, cu_of([3]), scale), slice(0, 3)), (dmm.paged_attention(q[2:], k, v, table, lens, scale), slice(2, 3))):
+            assert check_attention(got, want[rows], bound[rows]) == got.numel() and bool(torch.isfinite(got).all())
