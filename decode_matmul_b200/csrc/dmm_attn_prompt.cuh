@@ -505,11 +505,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     grid_dep_launch();  // (the kernel that joins parts waits for this one's end)
+    // What other warps may set at any time is read once for a warp: its lanes part nowhere, as what follows wants all of them.
+    const auto failed = [&]() { return __any_sync(0xffffffffu, s_failed) != 0; };
     // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.
     const auto item_of = [&](int k) {
         mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed);
         PromptItem it = s_item[k & 1];
-        if (s_failed) it.seq = -1;
+        if (failed()) it.seq = -1;
         return it;
     };
     const auto item_done = [&](int k) {
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 bool more = false;  // of this block's share
                 while (index >= 0) {
                     if (!shared || index < p.ctas) it = prompt_item(p, share, line, shared ? unit : index, unit_end, &unit);
-                    if (it.seq >= 0 || s_failed) break;
+                    if (it.seq >= 0 || failed()) break;
                     ask();  // (the grid has some blocks more than there is work for)
                     answer();
                 }
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     if (!more) crossing.ctas = 0;
                 }
                 if (k >= 2) mbar_wait(bar(Plan::kBarItemFree + (k & 1)), static_cast<uint32_t>((k >> 1) - 1) & 1u, &s_failed);
-                if (s_failed) it.seq = -1;
+                if (failed()) it.seq = -1;
                 if (lane == 0) {
                     s_item[k & 1] = it;
                     s_poison[k & 1] = 0;
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         mbar_wait(bar(Plan::kBarEmpty + stage), parity, &s_failed);
-                        if (s_failed) break;
+                        if (failed()) break;
                         // (values that the guard looks at first arrive at barriers of their own)
                         const uint32_t full = bar(kv == 1 && tile >= ext.guarded ? Plan::look(k, tile - ext.guarded) : Plan::kBarFull + stage);
                         if (lane == 0) mbar_arrive_expect_tx(full, bytes);
@@ -844,7 +846,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             float *const share = part ? prompt_slot(p, D, it.slot) + 128 * D * i : nullptr;
             if (part) *reinterpret_cast<float2 *>(prompt_slot(p, D, it.slot) + 256 * D + 2 * (128 * i + r)) = make_float2(m == -INFINITY ? m : m * c, l);
             T *const out = static_cast<T *>(p.out) + static_cast<long long>(it.begin + it.token0 + i * tt) * p.out_ld + static_cast<long long>(it.head * p.group) * D;
-            if (s_poison[k & 1]) {
+            // (a tile that waits for no products, or not for the later ones of the other tile, may come here while the guard looks: either way
+            // is right for it, but the warp's lanes go one way)
+            if (__any_sync(0xffffffffu, s_poison[k & 1])) {
                 // values that are not finite, which the guard has taken out of the tiles in which rows end: row by row
                 T *to = out + static_cast<long long>(tok) * p.out_ld + (r - tok * p.group) * D;
 #pragma unroll 1

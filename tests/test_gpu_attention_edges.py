@@ -68,3 +68,28 @@ def test_scores_of_millions(dtype):
         want, bound = attention(q, k, v, table, lens, cu_of([3]), scale)
         for got, rows in ((dmm.prompt_attention(q, k, v, table, lens, cu_of([3]), scale), slice(0, 3)), (dmm.paged_attention(q[2:], k, v, table, lens, scale), slice(2, 3))):
             assert check_attention(got, want[rows], bound[rows]) == got.numel() and bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("new,length,at", [(256, 256, 255), (256, 256, 130), (256, 100, 50), (250, 700, 640), (200, 30, 0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_value_that_only_the_second_tile_of_rows_sees(new, length, at, D):
+    """Two tiles of 128 rows are worked on together; the first is done, or has nothing to do, while the values that the second sees are
+    still looked at."""
+    gen = generator(6)
+    k, v, table, lens = make_cache(gen, [length] * 4, 64, D, 64, BF16)
+    q = torch.randn((4 * new, 64, D), generator=gen, device="cuda").to(BF16)
+    cu = cu_of([new] * 4)
+    want, bound = attention(q, k, v, table, lens, cu)
+    for b in (0, 1, 3):
+        v[int(table[b, at // 64]), :, at % 64, 9] = math.inf
+    sees = torch.arange(length - new, length, device="cuda") >= at
+    for _ in range(3):
+        got = dmm.prompt_attention(q, k, v, table, lens, cu)
+        rest = want.clone()
+        for b in (0, 1, 3):
+            rows = torch.nonzero(sees)[:, 0] + b * new
+            assert not bool(torch.isfinite(got[rows, :, 9]).any())
+            got[rows, :, 9] = 0
+            rest[rows, :, 9] = 0
+        assert check_attention(got, rest, bound) == got.numel()
+    assert dmm.status() == 0
