@@ -48,6 +48,7 @@ struct PromptParams {
 
 constexpr int kPromptThreads = 384;
 constexpr int kPromptKeys = 128;  // keys of a tile
+constexpr long long kPromptTileLimit = 20000;  // cycles that a wait allows for each of many key tiles: they take some 2800
 
 // Key tiles in which rows of a pair of tiles end: they are 256 tokens at most.
 constexpr int kMostGuarded = 3;
@@ -507,9 +508,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     grid_dep_launch();  // (the kernel that joins parts waits for this one's end)
     // What other warps may set at any time is read once for a warp: its lanes part nowhere, as what follows wants all of them.
     const auto failed = [&]() { return __any_sync(0xffffffffu, s_failed) != 0; };
-    // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.
-    const auto item_of = [&](int k) {
-        mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed);
+    // Most waits are for a step of a key tile; those of a warp that has nothing to do for an item may be as long as the item.
+    const auto limit_of = [](int tiles) { return kWaitLimitCycles + kPromptTileLimit * tiles; };
+    // The item of turn `k` for every warp but the one that finds them; no more when its sequence is -1.  `before`: key tiles of the item before.
+    const auto item_of = [&](int k, int before) {
+        mbar_wait(bar(Plan::kBarItem + (k & 1)), static_cast<uint32_t>(k >> 1) & 1u, &s_failed, limit_of(before));
         PromptItem it = s_item[k & 1];
         if (failed()) it.seq = -1;
         return it;
@@ -664,10 +667,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             Ring keys = {0, 0}, values = {1, 0};
             uint32_t q_full = 0, p_full = 0, o_free = 0, guard = 0, s_count = 0;  // bits: phases
             bool o_used[2] = {false, false};
-            for (int k = 0;; ++k) {
-                const PromptItem it = item_of(k);
+            for (int k = 0, before = 0;; ++k) {
+                const PromptItem it = item_of(k, before);
                 if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
+                before = ext.all;
                 // Scores and products go in the order (tile 0, key tile 0), (tile 1, 0), (0, 1), (1, 1), ...; the scores of two are asked
                 // for before the products of the first, and then always the next ones behind those of one more: they are there when
                 // a tile's softmax has done with the scores before.
@@ -757,14 +761,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             constexpr uint32_t kMask = F16Kind<T>::kExponent * 0x10001u;
             int tile0 = 0;        // tiles of the ring that items before had
             uint32_t look = 0;    // bits: phases
-            for (int k = 0;; ++k) {
-                const PromptItem it = item_of(k);
+            for (int k = 0, before = 0;; ++k) {
+                const PromptItem it = item_of(k, before);
                 if (it.seq < 0) break;
                 const PromptExtent ext(it, tt);
+                before = ext.all;
                 for (int j = max(0, ext.guarded - it.first); j < ext.all; ++j) {
                     // rows of values behind the first that not every query sees (or all of them, where the sequence ends)
                     const int rows = min(kPromptKeys, it.len - (it.first + j) * kPromptKeys), row0 = max(0, ext.seen - (it.first + j) * kPromptKeys), g = it.first + j - ext.guarded, at = Plan::phase_bit(k, g);
-                    mbar_wait(bar(Plan::look(k, g)), (look >> at) & 1u, &s_failed);
+                    mbar_wait(bar(Plan::look(k, g)), (look >> at) & 1u, &s_failed, limit_of(ext.all));
                     look ^= 1u << at;
                     const uint32_t base = smem + Plan::kRing + static_cast<uint32_t>((tile0 + 2 * j + 1) % Plan::kStages) * Plan::kTileBytes;
                     const auto where = [&](int c) { return base + (c / 1024) * Plan::kHalfBytes + (c % 1024) * 16u; };  // piece c: row (c % 1024) / 8
@@ -815,7 +820,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         // (the products have the sign of the scale; times 2^-149 every finite score is as good as 0, and a hidden one stays -infinity)
         const float c = p.scale == 0.0f ? __uint_as_float(1u) : fabsf(p.scale) * 1.4426950408889634f;
         uint32_t s_full = 0, o_full = 0, done = 0;  // phases
-        PromptItem next = item_of(0);
+        PromptItem next = item_of(0, 0);
         for (int k = 0;; ++k) {
             const PromptItem it = next;
             if (it.seq < 0) break;
@@ -835,7 +840,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (j > 0) done ^= 1u;
                 row.step(j >= free, m, l);
             }
-            next = item_of(k + 1);  // (known before this item's last products are done: its finding waits for none of them)
+            next = item_of(k + 1, ext.all);  // (known before this item's last products are done: its finding waits for none of them)
             if (tiles > 0) {
                 mbar_wait(bar(Plan::kBarO + i), o_full, &s_failed);
                 o_full ^= 1u;

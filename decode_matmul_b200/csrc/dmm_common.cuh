@@ -86,14 +86,14 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint32_t bar, uint32_t parity
     return ok != 0;
 }
 
-// Waits for a phase of an mbarrier, but never for longer than about a quarter of a second:
-// on expiry the CTA-wide `failed` flag is set, the device status word gets
+// Waits for a phase of an mbarrier, but never for longer than about a quarter of a second (`limit`
+// cycles): on expiry the CTA-wide `failed` flag is set, the device status word gets
 // DMM_STATUS_WAIT_TIMEOUT and every later wait of the CTA returns at once, so a lost
 // arrival produces a wrong result with a raised status instead of a hung GPU.
 constexpr long long kWaitLimitCycles = 500ll * 1000 * 1000;
 constexpr uint32_t kWaitHintNs = 20000;  // longest single suspension inside a wait
 
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *failed, long long limit = kWaitLimitCycles) {
     if (mbar_try_wait(bar, parity)) return;
     if (*failed) return;
     const long long t0 = clock64();
@@ -103,7 +103,7 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
 #pragma unroll 1
         for (int i = 0; i < 16; ++i)
             if (mbar_try_wait_hint(bar, parity, kWaitHintNs)) return;
-        if (clock64() - t0 > kWaitLimitCycles || *failed) {
+        if (clock64() - t0 > limit || *failed) {
             if (!*failed) {
                 *failed = 1;
                 raise_status(DMM_STATUS_WAIT_TIMEOUT);

@@ -93,3 +93,21 @@ def test_a_value_that_only_the_second_tile_of_rows_sees(new, length, at, D):
             rest[rows, :, 9] = 0
         assert check_attention(got, rest, bound) == got.numel()
     assert dmm.status() == 0
+
+
+def test_a_context_whose_item_takes_most_of_a_second():
+    """2^26 keys of every key head, all of them one page, and an item of one row for each CTA: warps that have nothing to do for it wait as
+    long as it takes."""
+    gen = generator(7)
+    n, page, heads = 2 ** 26, 4096, torch.cuda.get_device_properties(0).multi_processor_count
+    k = torch.randn((1, heads, page, 64), generator=gen, device="cuda").to(BF16)
+    v = (1.0 + 0.1 * torch.randn((1, heads, page, 64), generator=gen, device="cuda")).to(BF16)
+    table = torch.zeros((1, n // page), dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.randn((1, heads, 64), generator=gen, device="cuda").to(BF16)
+    got = dmm.prompt_attention(q, k, v, table, lens, cu_of([1]))
+    assert dmm.status() == 0
+    # every key is there 2^14 times, which is the same average.  The products add 16 keys at a time, 2^22 times, each off by a step of the
+    # sum at most, the sum of weights 128 at a time
+    want, bound = attention(q, k, v, table, lens.clamp(max=page), cu_of([1]))
+    assert check_attention(got, want, bound + (2.0 ** 22 * 2.0 ** -23 + 2.0 ** 19 * 2.0 ** -24) * want.abs()) == got.numel()
