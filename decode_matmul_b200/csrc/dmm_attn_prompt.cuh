@@ -30,6 +30,7 @@
 #pragma once
 
 #include "dmm_attn_common.cuh"
+#include "dmm_attn_item.h"
 #include "dmm_tmem.cuh"
 
 namespace dmm {
@@ -163,14 +164,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-
-// What a CTA works on: a pair of tiles of one key head, or a part of its key tiles.
-struct PromptItem {
-    int seq, head, begin, n, len, token0;  // token0: first token of tile 0 within the sequence's new tokens
-    int first, end;                        // key tiles
-    int slot;                              // of the workspace, for a part; -1 for the whole
-    int ctas;                              // for the first part: how many CTAs have one
-};
 
 constexpr int kPromptItem = 2;
 constexpr float kPromptJoin = 6.0f, kPromptLeast = 0.28f;  // 0.28 = sqrt(0.15 us a part in the join / 1.8 us a key tile)
@@ -543,7 +536,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (!shared || index < 0 || index >= p.ctas) return;
                 unit = share.begin(index);
                 unit_end = share.begin(index + 1);
-                if (unit == unit_end && lane == 0) prompt_crossings(p)[index] = crossing;  // (nothing)
+                if (lane == 0) prompt_crossings(p)[index] = crossing;  // (nothing, until the share is done)
             };
             const auto ask = [&]() {
                 if (lane == 0) ask_next_block(smem_u32(s_answer), bar(Plan::kBarNext));
@@ -552,7 +545,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const auto answer = [&]() {
                 mbar_wait(bar(Plan::kBarNext), asked & 1u, &s_failed);
                 ++asked;
-                index = next_block(smem_u32(s_answer));
+                index = failed() ? -1 : next_block(smem_u32(s_answer));  // (without an answer there is no block)
                 __syncwarp();
                 begin_block();
             };
@@ -952,7 +945,7 @@ __global__ void __launch_bounds__(8 * kJoinRows) prompt_join_kernel(const Prompt
     grid_dep_wait();
     if (reinterpret_cast<const PromptHead *>(p.workspace)->shared == 0) return;
     const PromptItem it = prompt_crossings(p)[blockIdx.y];
-    if (it.ctas == 0) return;
+    if (!prompt_item_crosses(it, static_cast<int>(blockIdx.y), p.ctas, p.cache.kv_heads, p.tokens)) return;
     const auto slot = [&](int s) { return prompt_slot(p, D, s == 0 ? it.slot : 2 * (static_cast<int>(blockIdx.y) + s)); };
     constexpr int kPieces = D / 32;  // of four columns, 32 columns apart
     const int row = static_cast<int>(blockIdx.x) * kJoinRows + static_cast<int>(threadIdx.x) / 8;
