@@ -117,7 +117,8 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
 
     ``qkv`` is fp32, fp16 or bf16 [tokens, (heads + 2 kv_heads) * head_dim]: query heads, key heads, value heads.  Rows
     ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32 [sequences + 1]) are the last tokens of sequence b, whose
-    ``seq_lens[b]`` counts them; without ``cu_seqlens`` there is one token per sequence.  Queries and keys are rotated by
+    ``seq_lens[b]`` counts them; without ``cu_seqlens`` there is one token per sequence, and the row of a sequence of length 0 is
+    skipped.  Queries and keys are rotated by
     their position times ``freqs`` (float64 [head_dim / 2], :func:`rotary_frequencies`; None: not rotated), the two
     halves of a head as pairs or, ``interleaved``, neighbours.  Rows behind the last sequence are skipped.  No two tokens
     of a call may have the same place in the cache; ``output`` may be the query heads of a 16-bit ``qkv`` themselves."""

@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendP
     if (b < 0) return;
     const TokenSpan span = token_span(p.cu, b, p.tokens);
     const int pos = cache_len(p.cache, b) - span.n + (t - span.begin);
-    if (pos < 0) {
-        raise_status(DMM_STATUS_BAD_PAGE);
+    if (pos < 0) {  // (without cu: a sequence that has no tokens, whose place in the batch is idle)
+        if (p.cu != nullptr) raise_status(DMM_STATUS_BAD_PAGE);
         return;
     }
     if (p.freqs != nullptr && threadIdx.x < D / 2) {

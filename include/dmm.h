@@ -373,7 +373,8 @@ typedef struct dmm_paged_cache {
  * The result of a qkv product becomes queries, and new rows of the cache.  qkv: [tokens, qkv_ld] of qkv_type (fp32, fp16 or
  * bf16), a row = `heads` query heads, then kv_heads key heads, then kv_heads value heads of head_dim values.  The tokens of
  * sequence b are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 and its last ones: token i of n has position
- * seq_lens[b] - n + i.  cu_seqlens (int32 [num_seqs + 1]) may be NULL: one token per sequence, row b.
+ * seq_lens[b] - n + i.  cu_seqlens (int32 [num_seqs + 1]) may be NULL: one token per sequence, row b; a sequence of length 0 has
+ * an idle place then, and its row is skipped.
  * Queries and keys are rotated by their position: freqs[i] (double, head_dim / 2 of them, device memory) is the angle
  * in radians per position of pair i, (a, b) -> (a cos - b sin, a sin + b cos); a pair is (i, i + head_dim / 2), or
  * (2 i, 2 i + 1) with `interleaved`.  freqs NULL: no rotation.  The angle is reduced in 64 bits, the rotation is done in 32

@@ -111,3 +111,24 @@ def test_a_context_whose_item_takes_most_of_a_second():
     # sum at most, the sum of weights 128 at a time
     want, bound = attention(q, k, v, table, lens.clamp(max=page), cu_of([1]))
     assert check_attention(got, want, bound + (2.0 ** 22 * 2.0 ** -23 + 2.0 ** 19 * 2.0 ** -24) * want.abs()) == got.numel()
+
+
+def test_a_sequence_without_tokens_has_an_idle_place_in_a_batch():
+    """Without cu_seqlens every sequence has a row; that of an empty one is left alone and raises nothing."""
+    gen = generator(5)
+    k, v, table, lens = make_cache(gen, [20, 0, 33, 0], 2, 64, 16, FP16)
+    k0, v0 = k.clone(), v.clone()
+    qkv = torch.randn((4, 8 * 64), generator=gen, device="cuda")
+    qkv[1::2] = math.nan
+    q = torch.full((4, 4, 64), math.nan, dtype=FP16, device="cuda")
+    dmm.append_kv(qkv, k, v, table, lens, dmm.rotary_frequencies(64, device="cuda"), q)
+    assert dmm.status() == 0 and bool(torch.isnan(q[1::2]).all()) and bool(torch.isfinite(q[::2]).all())
+    for b, n in ((0, 20), (2, 33)):
+        at = int(table[b, (n - 1) // 16]), slice(None), (n - 1) % 16
+        assert torch.equal(v[at], qkv[b].view(8, 64)[6:].to(FP16))
+        k0[at], v0[at] = k[at], v[at]
+    assert torch.equal(k.view(torch.int16), k0.view(torch.int16)) and torch.equal(v.view(torch.int16), v0.view(torch.int16))
+    got = dmm.paged_attention(q, k, v, table, lens)
+    assert dmm.status() == 0 and bool((got[1::2] == 0).all())
+    want, bound = attention(torch.nan_to_num(q), k, v, table, lens, None)
+    assert check_attention(got, want, bound) == got.numel()
