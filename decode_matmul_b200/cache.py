@@ -48,13 +48,19 @@ class PagedCache:
     def free_pages(self) -> int:
         return len(self._free)
 
-    def extend(self, new) -> torch.Tensor | None:
+    def extend(self, new, *, idle: bool = False) -> torch.Tensor | None:
         """Makes room for ``new[b]`` tokens at the end of every sequence and counts them in.  Returns the ``cu_seqlens`` of
         their rows, packed in the order of the sequences, or None when every sequence has one.  Raises without having
-        changed anything when pages run out."""
+        changed anything when pages run out.
+
+        ``idle``: sequences that have no tokens, such as those that :meth:`release` has ended, sit out a step of one token for each of the
+        others (``new[b]`` is 0 for them, 1 for the others).  Returns None: every sequence has a row, which counts for nothing where
+        the sequence is empty.  A captured step of single tokens so goes on while sequences come and go."""
         new = [int(n) for n in new]
         if len(new) != self.max_seqs or min(new) < 0:
             raise RuntimeError(f"new must be {self.max_seqs} numbers of tokens")
+        if idle and any(n > 1 or (n == 0 and length > 0) for n, length in zip(new, self.lengths)):
+            raise RuntimeError("with idle, new must be 1, or 0 for sequences without tokens")
         want = [-(-(length + n) // self.page_size) - len(own) for length, n, own in zip(self.lengths, new, self._owned)]
         if any(len(own) + w > self.max_pages for own, w in zip(self._owned, want)):
             raise RuntimeError(f"a sequence is longer than {self.max_pages} pages of {self.page_size} tokens")
@@ -70,6 +76,8 @@ class PagedCache:
             self.seq_lens += 1
             return None
         self.seq_lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+        if idle:
+            return None
         ends = torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32)
         return ends.to(self.device)
 

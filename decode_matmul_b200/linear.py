@@ -131,7 +131,7 @@ class LinearStack:
 
         ``cache`` (a :class:`PagedCache` of this rank's key heads, fp16): the blocks attend.  The rows of ``h`` are the new
         tokens of its sequences, for which :meth:`PagedCache.extend` has made room; ``cu_seqlens`` is what that returned, None
-        for one token per sequence.  Rows behind the last sequence pass the blocks without attention.
+        for one token per sequence.  Rows behind the last sequence, and those of sequences without tokens, pass the blocks without attention.
 
         ``fused`` (default: whenever the batch is at most 32): every elementwise step between two
         layers runs inside the matmul kernels -- the loaders read fp32 and round to fp16 or form

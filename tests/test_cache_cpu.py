@@ -236,3 +236,22 @@ def test_rotary_frequencies():
     assert torch.allclose(f, 500.0 ** (-torch.arange(64, dtype=torch.float64) / 64), rtol=1e-15)
     with pytest.raises(RuntimeError):
         dmm.rotary_frequencies(7)
+
+
+def test_idle_sequences_sit_out_a_step():
+    c = make()
+    c.extend([15, 3, 16])
+    c.release(1)
+    assert c.extend([1, 0, 1], idle=True) is None
+    assert c.lengths == [16, 0, 17] and c.seq_lens.tolist() == [16, 0, 17] and c.free_pages == 4
+    used = table_of(c, 0) + table_of(c, 2)
+    assert len(used) == len(set(used)) == 3
+    before = (list(c.lengths), c.free_pages, c.page_table.clone(), c.seq_lens.clone())
+    for new in ([0, 0, 1], [1, 2, 1], [2, 0, 1]):  # a sequence that has tokens would get one; more than one token
+        with pytest.raises(RuntimeError, match="idle"):
+            c.extend(new, idle=True)
+        assert (c.lengths, c.free_pages) == before[:2] and torch.equal(c.page_table, before[2]) and torch.equal(c.seq_lens, before[3])
+    assert c.extend([1, 1, 1], idle=True) is None and c.seq_lens.tolist() == [17, 1, 18]
+    assert c.extend([1, 0, 1]).tolist() == [0, 1, 1, 2]  # without it rows are packed, as ever
+    c = make()
+    assert c.extend([0, 0, 0], idle=True) is None and c.free_pages == 7

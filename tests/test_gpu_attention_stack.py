@@ -204,3 +204,41 @@ def test_the_first_step_with_a_cache_is_not_captured():
     with pytest.raises(RuntimeError, match="cannot be captured"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             stack.step(h, cache=cache)
+
+
+def test_a_captured_step_goes_on_while_sequences_come_and_go():
+    """One of three sequences ends between replays and another takes its place: the others' rows are what they are without it."""
+    stack, cache, twin = stack_of(CFG), cache_of(CFG), cache_of(CFG)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    start = torch.randn((3 * 20, CFG["hidden"]), generator=gen, device="cuda")
+    for c in (cache, twin):
+        stack.step(start.clone(), cache=c, cu_seqlens=c.extend([20, 20, 20]))
+    h = torch.zeros((3, CFG["hidden"]), device="cuda")
+    cache.extend([1, 1, 1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        stack.step(h, cache=cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stack.step(h, cache=cache)
+    cache.seq_lens -= 1
+    cache.lengths = [n - 1 for n in cache.lengths]
+    for i in range(12):
+        if i == 3:
+            cache.release(1)
+            twin.release(1)
+        if i == 8:  # (a new prompt comes in)
+            rows = torch.randn((9, CFG["hidden"]), generator=gen, device="cuda")
+            for c in (cache, twin):
+                stack.step(rows.clone(), cache=c, cu_seqlens=c.extend([0, 9, 0]))
+        new = [1, 0, 1] if 3 <= i < 8 else [1, 1, 1]
+        x = torch.randn((3, CFG["hidden"]), generator=gen, device="cuda")
+        assert cache.extend(new, idle=True) is None
+        h.copy_(x)
+        graph.replay()
+        live = torch.tensor([b for b in range(3) if new[b]], device="cuda")
+        near(h[live], stack.step(x[live], cache=twin, cu_seqlens=twin.extend(new)), 2 * CFG["layers"])
+        assert bool(torch.isfinite(h).all()) and torch.equal(cache.seq_lens, twin.seq_lens)
+    assert dmm.status() == 0
