@@ -2,7 +2,8 @@
 
 The library has two translation units, csrc/dmm_api.cu (the products) and csrc/dmm_attn_api.cu (attention), which
 include the kernel headers and are compiled side by side; the result is written next to this file so that it travels
-with the source tree.  The object files stay there too, and one whose sources have not changed is taken as it is.
+with the source tree.  The object files stay there too, and one is taken as it is when its sources have not changed and
+the same compiler would make it with the same command (an ``.o.cmd`` beside it says which did).
 """
 from __future__ import annotations
 
@@ -44,6 +45,15 @@ def _depends(path, seen=None):
     return seen
 
 
+def _made_by(obj) -> str | None:
+    """What an object file was made with, None when nothing says so."""
+    try:
+        with open(obj + ".cmd") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
@@ -67,21 +77,28 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if not force and not needs_build():
                 return LIB
             nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+            version = subprocess.run([nvcc, "--version"], capture_output=True, text=True).stdout
             objects, running, log = [], [], ""
             for unit in UNITS:
                 source = os.path.join(CSRC, unit)
                 obj = source[:-3] + ".o"
                 objects.append(obj)
-                if not force and os.path.exists(obj) and all(os.path.getmtime(s) <= os.path.getmtime(obj) for s in _depends(source)):
+                made_by = "\n".join([nvcc, *NVCC_FLAGS, unit, version])
+                if (not force and os.path.exists(obj) and _made_by(obj) == made_by
+                        and all(os.path.getmtime(s) <= os.path.getmtime(obj) for s in _depends(source))):
                     continue
+                if os.path.exists(obj + ".cmd"):
+                    os.remove(obj + ".cmd")
                 tmp = f"{obj}.{os.getpid()}.tmp"
                 cmd = [nvcc, *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-c", "-o", tmp, source]
-                running.append((obj, tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+                running.append((obj, tmp, made_by, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
             failed = False
-            for obj, tmp, proc in running:
+            for obj, tmp, made_by, proc in running:
                 log += proc.communicate()[0]
                 if proc.returncode == 0:
                     os.replace(tmp, obj)
+                    with open(obj + ".cmd", "w") as f:
+                        f.write(made_by)
                     continue
                 failed = True
                 if os.path.exists(tmp):
