@@ -30,8 +30,8 @@ class PagedCache:
         self.max_seqs, self.max_pages = max_seqs, num_pages if max_pages is None else max_pages
         if self.max_pages < 1:
             raise RuntimeError("max_pages must be positive")
-        self.device = torch.device(device)
-        self.pages = torch.zeros((layers, 2, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=self.device)
+        self.pages = torch.zeros((layers, 2, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.device = self.pages.device  # ("cuda" alone is whichever device is current when it is used)
         self.page_table = torch.zeros((max_seqs, self.max_pages), dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros((max_seqs,), dtype=torch.int32, device=self.device)
         self.lengths = [0] * max_seqs

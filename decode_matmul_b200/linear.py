@@ -76,7 +76,7 @@ class LinearStack:
                  tp_mode: str | None = None):
         self.cfg, self.world, self.rank, self.group = cfg, world, rank, group
         self.tp_mode = tp_mode  # None: by rank count and DMM_TP_MODE; "slots" | "pull" | "push" | "nccl"
-        self.device = torch.device(device)
+        self.device = torch.empty((0,), device=device).device  # ("cuda" alone is whichever device is current when it is used)
         self.hidden, self.ffn = cfg["hidden"], cfg["ffn"]
         shapes = llama_shapes(cfg["hidden"], cfg["kv_heads"], cfg["head_dim"], cfg["ffn"])
         for name, (n, k) in shapes.items():

@@ -7,6 +7,7 @@ import torch
 
 import decode_matmul_b200 as dmm
 from attention_reference import attention, check_attention, gather
+from decode_matmul_b200.linear import LinearStack
 from test_gpu_attention import cu_of, generator, make_cache
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +133,11 @@ def test_a_sequence_without_tokens_has_an_idle_place_in_a_batch():
     assert dmm.status() == 0 and bool((got[1::2] == 0).all())
     want, bound = attention(torch.nan_to_num(q), k, v, table, lens, None)
     assert check_attention(got, want, bound) == got.numel()
+
+
+def test_caches_and_stacks_know_their_device():
+    # "cuda" is whichever device is current at the time
+    here = torch.device("cuda", torch.cuda.current_device())
+    assert dmm.PagedCache(1, 1, 64, 2, device="cuda").device == here
+    cb = dmm.codebook_to_fp16(dmm.pack_codebook(dmm.synthetic_codebook(42)))
+    assert LinearStack(dict(hidden=256, kv_heads=2, head_dim=64, ffn=256, layers=1), cb, "cuda").device == here
