@@ -45,6 +45,8 @@ def _check_cache(k, v, table, lens):
     if len(shape) != 4:
         _no("k_pages must be [num_pages, kv_heads, page_size, head_dim]")
     pages, kv_heads, page_size, head_dim = shape
+    if not pages or not kv_heads:
+        _no("k_pages must not be empty")
     if head_dim != 128 and head_dim != 64:
         _no("head_dim must be 64 or 128")
     if page_size < 16 or page_size & (page_size - 1):

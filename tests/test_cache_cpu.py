@@ -255,3 +255,14 @@ def test_idle_sequences_sit_out_a_step():
     assert c.extend([1, 0, 1]).tolist() == [0, 1, 1, 2]  # without it rows are packed, as ever
     c = make()
     assert c.extend([0, 0, 0], idle=True) is None and c.free_pages == 7
+
+
+@pytest.mark.parametrize("shape", [(9, 0, 16, 64), (0, 2, 16, 64)])
+def test_an_empty_cache_is_refused(calls, shape):
+    _, _, table, lens = cache_of()
+    k, v = dev(shape, torch.float16), dev(shape, torch.float16)
+    with pytest.raises(RuntimeError, match="empty"):
+        dmm.paged_attention(dev((2, 8, 64), torch.float16), k, v, table, lens)
+    with pytest.raises(RuntimeError, match="empty"):
+        dmm.append_kv(dev((2, 512), torch.float32), k, v, table, lens)
+    assert not calls
