@@ -172,6 +172,8 @@ class LinearStack:
         from .ops import decode_matmul_sequence, fused_op
 
         head_dim, kv_heads = self.cfg["head_dim"], self.cfg["kv_heads"] // self.world
+        if self.cfg["kv_heads"] % self.world or self.hidden % (self.cfg["kv_heads"] * head_dim):
+            raise RuntimeError(f"{self.cfg['kv_heads']} key heads of {head_dim} and as many groups of query heads in {self.hidden} do not shard over {self.world} ranks")
         if cache.layers != len(self.layers) or cache.kv_heads != kv_heads or cache.head_dim != head_dim or cache.pages.dtype != torch.float16:
             raise RuntimeError(f"cache must be fp16, of {len(self.layers)} layers with {kv_heads} key heads of {head_dim}")
         if getattr(self, "_freqs", None) is None:
