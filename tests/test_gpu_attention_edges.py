@@ -71,6 +71,51 @@ def test_scores_of_millions(dtype):
             assert check_attention(got, want[rows], bound[rows]) == got.numel() and bool(torch.isfinite(got).all())
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("group", [1, 8, 12])
+def test_one_value_of_one_sequence_of_a_batch(what, dtype, group):
+    """Sequences that a warp has whole, that a CTA's warps join, and that CTAs join: one element of one value shows in its column of
+    the heads that read it, and nowhere else."""
+    gen = generator(3)
+    lens_ = [17, 3, 400, 1, 30000, 250, 0, 16]
+    k, v, table, lens = make_cache(gen, lens_, 2, 128, 16, dtype)
+    q = torch.randn((len(lens_), 2 * group, 128), generator=gen, device="cuda").to(dtype)
+    want, bound = attention(q, k, v, table, lens, None)
+    for seq, pos in ((0, 0), (0, 16), (2, 399), (4, 0), (4, 15003), (4, 29999), (7, 15)):
+        at = (int(table[seq, pos // 16]), 1, pos % 16, 77)
+        kept = v[at].clone()
+        v[at] = what
+        got = dmm.paged_attention(q, k, v, table, lens)
+        v[at] = kept
+        assert not bool(torch.isfinite(got[seq, group:, 77]).any())
+        mended, rest = got.clone(), want.clone()
+        mended[seq, group:, 77] = 0
+        rest[seq, group:, 77] = 0
+        assert check_attention(mended, rest, bound) == got.numel()
+    assert dmm.status() == 0
+
+
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+def test_a_key_that_is_not_finite_shows_in_the_rows_that_see_it(what):
+    # against queries of either sign its score is inf - inf
+    gen = generator(4)
+    k, v, table, lens = make_cache(gen, [200, 30], 2, 128, 16, FP16)
+    q = torch.randn((230, 16, 128), generator=gen, device="cuda").to(FP16)
+    want, bound = attention(q, k, v, table, lens, cu_of([200, 30]))
+    k[int(table[0, 70 // 16]), 1, 70 % 16] = what
+    got = dmm.prompt_attention(q, k, v, table, lens, cu_of([200, 30]))
+    assert not bool(torch.isfinite(got[70:200, 8:]).any())
+    got[70:200, 8:] = 0
+    want[70:200, 8:] = 0
+    assert check_attention(got, want, bound) == got.numel()
+    last = torch.tensor([199, 229], device="cuda")
+    one = dmm.paged_attention(q[last], k, v, table, lens)
+    assert not bool(torch.isfinite(one[0, 8:]).any())
+    one[0, 8:] = 0
+    assert check_attention(one, want[last], bound[last]) == one.numel()
+
+
 @pytest.mark.parametrize("new,length,at", [(256, 256, 255), (256, 256, 130), (256, 100, 50), (250, 700, 640), (200, 30, 0)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_value_that_only_the_second_tile_of_rows_sees(new, length, at, D):
