@@ -120,9 +120,8 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
     ``qkv`` is fp32, fp16 or bf16 [tokens, (heads + 2 kv_heads) * head_dim]: query heads, key heads, value heads.  Rows
     ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` (int32 [sequences + 1]) are the last tokens of sequence b, whose
     ``seq_lens[b]`` counts them; without ``cu_seqlens`` there is one token per sequence, and the row of a sequence of length 0 is
-    skipped.  Queries and keys are rotated by
-    their position times ``freqs`` (float64 [head_dim / 2], :func:`rotary_frequencies`; None: not rotated), the two
-    halves of a head as pairs or, ``interleaved``, neighbours.  Rows behind the last sequence are skipped.  No two tokens
+    skipped.  Queries and keys are rotated by their position times ``freqs`` (float64 [head_dim / 2],
+    :func:`rotary_frequencies`; None: not rotated), the two halves of a head as pairs or, ``interleaved``, neighbours.  Rows behind the last sequence are skipped.  No two tokens
     of a call may have the same place in the cache; ``output`` may be the query heads of a 16-bit ``qkv`` themselves."""
     cache, dtype, index, kv_heads, head_dim, seqs = _check_cache(k_pages, v_pages, page_table, seq_lens)
     kind = _TYPE_IN.get(qkv.dtype) if isinstance(qkv, torch.Tensor) else None
@@ -173,8 +172,8 @@ def append_kv(qkv, k_pages, v_pages, page_table, seq_lens, freqs=None, output=No
 
 
 def attention_workspace_bytes(tokens: int, sequences: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    """Bytes of scratch a call of :func:`paged_attention` (tokens = sequences) or :func:`prompt_attention` needs on the
-    current device (``dmm_attention_workspace_bytes``)."""
+    """Bytes of scratch that calls of :func:`paged_attention` (tokens = sequences) or :func:`prompt_attention` need on the
+    current device, for any lengths; at present ``head_dim`` alone decides (``dmm_attention_workspace_bytes``)."""
     return int(_lib.lib().dmm_attention_workspace_bytes(tokens, sequences, heads, kv_heads, head_dim))
 
 
@@ -235,9 +234,10 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, scale=None, outpu
 
     ``q`` is [sequences, heads, head_dim]; query head h reads key head h // (heads / kv_heads), over the ``seq_lens[b]``
     keys of its sequence.  ``scale`` defaults to head_dim ** -0.5.  A sequence of length 0 gets zeros.  Sequences may share pages.
-    ``workspace``: scratch
-    of at least :func:`attention_workspace_bytes` bytes, not shared with calls that may overlap on the GPU; by default the
-    call allocates its own."""
+    The weights of the softmax are rounded to the cache's type before they multiply the values; scores, maxima and sums are fp32.
+    ``output`` shares no memory with q, the cache or the workspace.  ``workspace``: scratch of at least
+    :func:`attention_workspace_bytes` bytes, not shared with calls that may overlap on the GPU; by default the call allocates
+    its own."""
     return _attend("paged_attention", q, k_pages, v_pages, page_table, seq_lens, None, scale, output, workspace, pdl)
 
 

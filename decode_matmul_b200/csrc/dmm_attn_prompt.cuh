@@ -23,10 +23,11 @@
 // cycles for their 32768 exponentials (16 a cycle).  Neither is reached: a step of a tile's softmax takes some 2000 cycles of a warp (scores
 // into registers, the maximum, the exponentials, of which two tiles' share the unit) and waits some 800 for products, and two tiles of
 // a CTA are all that tensor memory holds.
-// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 856 us (1.28 PFLOP/s, 77 % of what a dense product reaches; tensor
+// B200, graph, fp16, 64 heads of 128 on 8: 8192 tokens 864 us (1.27 PFLOP/s, 77 % of what a dense product reaches; tensor
 // pipe 65 % busy, exponentials 65 %), 2048 tokens 70 us (0.98 PFLOP/s): every item has a beginning (its first keys' way from HBM, the
 // guard) and an end (the last P V, O to memory) of 3 to 4 us that only the next item's loads run beside.  Under a load of some seconds
-// the clock falls to 1.6 GHz at the power cap, and 8192 tokens take 970 to 990 us.
+// the power cap takes the clock to 1.53 to 1.73 GHz, and 8192 tokens take 1004 us, 2048 81.  With 64 values a head the exponentials are the bound, at
+// twice the products' cycles: 8192 tokens 692 us (477 of exponentials), 2048 65 (30).
 #pragma once
 
 #include "dmm_attn_common.cuh"
@@ -200,9 +201,10 @@ __device__ __forceinline__ float warp_sum(float x) {
 //               kPromptJoin key tiles, and longer the more parts an item has: shares are no smaller than kPromptLeast
 //               times the square root of the longest item, and CTAs without one stay idle.
 // Which of the two ends sooner is estimated: whole items end with the longest, or half of the shortest of a sequence (on
-// average over the work) behind an even share.  B200, whole items against even shares: measured with two copies of a softmax step in the code, a prompt of 2048 tokens 74 us against
-// 131, of 8192 869 against 1660 (an item counts as the longest of its sequence), of 1024 with 8 heads 23 against 28; four chunks of 33 to
-// 512 tokens behind 511 to 16384 238 against 185; 16 tokens of 8 heads behind 16384 164 against 34.
+// average over the work) behind an even share.  B200, whole items against even shares: a prompt of 2048 tokens 76 us against
+// 131, of 8192 891 against 1535 (an item counts as the longest of its sequence); on 8 heads and one key head 1024 tokens 22.8 against 25.1, 2048 36.7
+// against 33.6, 4096 67 against 71, 8192 126 against 213; four chunks of 33 to 512 tokens behind 511 to 16384 262 against 190; 8 heads behind
+// long contexts 16 tokens behind 16384 169 against 36, 512 behind 8192 125 against 40.
 struct PromptShare {
     int each, more, all;
     __device__ __forceinline__ int begin(int x) const { return min(each * x + min(x, more), all); }

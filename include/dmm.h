@@ -393,7 +393,9 @@ int dmm_append_kv(const void *qkv, int qkv_type, int64_t qkv_ld, int64_t tokens,
  * over the keys j < seq_lens[b], group = heads / kv_heads (at most 128).  q and out: [num_seqs, heads, head_dim] of
  * the cache's type, q_ld / out_ld elements from one sequence to the next (multiples of 8), 16-byte aligned.  A sequence
  * of length 0 gets zeros, and so does a row whose scores are all -infinity; otherwise values that are not finite show in the rows
- * that see them, and in no others.  out shares no memory with q or the cache; sequences may share pages.  The keys of all sequences are cut into equal shares, one per CTA; what shares of one sequence
+ * that see them, and in no others.  The weights of the softmax are rounded to the cache's type before they multiply the values, half a step
+ * each (fp16 weights are held 2^7 up, so that light ones count); scores, maxima and sums are fp32, and the result is rounded once.
+ * out shares no memory with q, the cache or the workspace; sequences may share pages.  The keys of all sequences are cut into equal shares, one per CTA; what shares of one sequence
  * have in common is joined in a fixed order, so equal inputs give equal bits.  workspace: scratch of
  * dmm_attention_workspace_bytes, 256-byte aligned, of any content; calls that can overlap on the GPU need distinct ones.
  * flags: DMM_FLAG_PDL only.
@@ -405,13 +407,17 @@ int dmm_paged_attention(const void *q, int64_t q_ld, int heads, float scale, voi
  * Causal attention of packed prompts, or of the next chunk of each: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q
  * are the last tokens of sequence b, and row i of n sees the keys j <= seq_lens[b] - n + i, all of which are in the cache
  * (dmm_append_kv has put the new ones there).  A row that sees no key gets zeros; rows behind the last sequence are left
- * as they are.  Everything else as in dmm_paged_attention.
+ * as they are.  With a scale of 0 a score of -infinity before scaling hides its key instead of making the row NaN.  Everything else
+ * as in dmm_paged_attention.
  */
 int dmm_prompt_attention(const void *q, int64_t q_ld, int64_t tokens, int heads, float scale, void *out, int64_t out_ld,
                          const dmm_paged_cache *cache, const int32_t *cu_seqlens, void *workspace,
                          size_t workspace_bytes, unsigned flags, void *stream);
 
-/* Bytes of workspace that dmm_paged_attention (tokens = num_seqs) and dmm_prompt_attention need, for any lengths. */
+/*
+ * Bytes of workspace that dmm_paged_attention (tokens = num_seqs) and dmm_prompt_attention need on the current device, for any
+ * lengths.  At present they depend on head_dim and the device alone.
+ */
 size_t dmm_attention_workspace_bytes(int64_t tokens, int num_seqs, int heads, int kv_heads, int head_dim);
 
 /* Bytes of workspace a call of dmm_i8 / dmm_f16 with these sizes needs (0 if none). */
